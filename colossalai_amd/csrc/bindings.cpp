@@ -57,6 +57,10 @@ c10::optional<at::Tensor> native_flash_attention_varlen(const at::Tensor& q, con
 c10::optional<at::Tensor> native_fused_rope_attention(const at::Tensor& qkv, const at::Tensor& table,
                                                       const c10::optional<at::Tensor>& positions, int64_t Hq, int64_t Hkv,
                                                       int64_t D, bool causal, double scale, const c10::optional<at::Tensor>& seqlens);
+c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> native_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk,
+                                                                               const at::Tensor& table,
+                                                                               const c10::optional<at::Tensor>& positions, int64_t Hq,
+                                                                               int64_t Hkv, double eps);
 
 // layernorm.hip
 std::vector<at::Tensor> layernorm_fwd(at::Tensor input, at::Tensor gamma, c10::optional<at::Tensor> beta,
@@ -67,6 +71,12 @@ std::vector<at::Tensor> layernorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor ga
 // rope.hip
 void rope_inplace(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor table,
                   c10::optional<at::Tensor> positions, bool backward);
+
+// norm_rope.hip
+std::vector<at::Tensor> norm_rope_fwd(at::Tensor qkv, at::Tensor wq, at::Tensor wk, at::Tensor table, c10::optional<at::Tensor> positions,
+                                      int64_t Hq, int64_t Hkv, double eps);
+std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq, at::Tensor dk, at::Tensor dv, at::Tensor qkv, at::Tensor wq, at::Tensor wk,
+                                      at::Tensor table, c10::optional<at::Tensor> positions, int64_t Hq, int64_t Hkv, double eps);
 
 // swiglu.hip
 at::Tensor swiglu_fwd(at::Tensor gate_up);
@@ -146,6 +156,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("native_flash_attention", &cai::native_flash_attention);
   m.def("native_flash_attention_varlen", &cai::native_flash_attention_varlen);
   m.def("native_fused_rope_attention", &cai::native_fused_rope_attention);
+  m.def("native_norm_rope", &cai::native_norm_rope);
+  m.def("norm_rope_fwd", &cai::norm_rope_fwd, "packed projection: heads split, queries and keys normed and rotated");
+  m.def("norm_rope_bwd", &cai::norm_rope_bwd, "norm_rope_fwd backward: gradients of the projection and both weights");
   m.def("layernorm_fwd", &cai::layernorm_fwd, "LayerNorm forward");
   m.def("layernorm_bwd", &cai::layernorm_bwd, "LayerNorm backward");
   m.def("rope_inplace", &cai::rope_inplace, "in-place rotary embedding (fwd/bwd)");

@@ -13,6 +13,10 @@ std::vector<at::Tensor> rmsnorm_fused_add_fwd(at::Tensor input, at::Tensor resid
                                               bool save_inv_rms, c10::optional<at::Tensor> res_out);
 std::vector<at::Tensor> rmsnorm_bwd(at::Tensor dy, at::Tensor x, at::Tensor weight, at::Tensor inv_rms,
                                     c10::optional<at::Tensor> dres, bool cast_dw);
+std::vector<at::Tensor> norm_rope_fwd(at::Tensor qkv, at::Tensor wq, at::Tensor wk, at::Tensor table, c10::optional<at::Tensor> positions,
+                                      int64_t Hq, int64_t Hkv, double eps);
+std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq, at::Tensor dk, at::Tensor dv, at::Tensor qkv, at::Tensor wq, at::Tensor wk,
+                                      at::Tensor table, c10::optional<at::Tensor> positions, int64_t Hq, int64_t Hkv, double eps);
 at::Tensor swiglu_fwd(at::Tensor gate_up);
 at::Tensor swiglu_bwd(at::Tensor dout, at::Tensor gate_up);
 void rope_inplace(at::Tensor q, c10::optional<at::Tensor> k, at::Tensor table, c10::optional<at::Tensor> positions, bool backward);
@@ -148,6 +152,50 @@ struct FusedRopeAttention : torch::autograd::Function<FusedRopeAttention> {
   }
 };
 
+// y of norm_rope.hip in operations that autograd knows
+at::Tensor norm_rope_known(const at::Tensor& x, const at::Tensor& w, const at::Tensor& table, const Maybe& positions, double eps) {
+  const int64_t half = x.size(3) / 2;
+  const at::Tensor f = x.to(at::kFloat);
+  const at::Tensor y = f * at::rsqrt(f.square().mean(-1, true) + eps) * w.to(at::kFloat);
+  const at::Tensor rows = positions ? table.index_select(0, positions->reshape(-1)).view({x.size(0), x.size(1), 1, -1})
+                                    : table.slice(0, 0, x.size(1)).view({1, x.size(1), 1, -1});
+  const at::Tensor c = rows.narrow(3, 0, half), s = rows.narrow(3, half, half), lo = y.narrow(3, 0, half), hi = y.narrow(3, half, half);
+  return at::cat({lo * c - hi * s, hi * c + lo * s}, -1).to(x.scalar_type());
+}
+
+struct NormRope : torch::autograd::Function<NormRope> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk,
+                               const at::Tensor& table, const Maybe& positions, int64_t Hq, int64_t Hkv, double eps) {
+    auto r = norm_rope_fwd(qkv, wq, wk, table, positions, Hq, Hkv, eps);
+    ctx->saved_data["heads"] = std::vector<int64_t>{Hq, Hkv};
+    ctx->saved_data["eps"] = eps;
+    ctx->save_for_backward({qkv, wq, wk, table, positions.value_or(none)});
+    return {r[0], r[1], r[2]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["heads"].toIntVector();
+    const double eps = ctx->saved_data["eps"].toDouble();
+    if (at::GradMode::is_enabled()) {  // the gradient is part of a graph itself: the kernel's result would end it
+      const Heads h(s[0], n[0], n[1], s[1].numel());
+      const variable_list of = {s[0], s[1], s[2]},
+          out = {norm_rope_known(h.q, s[1], s[3], maybe(s[4]), eps), norm_rope_known(h.k, s[2], s[3], maybe(s[4]), eps), h.v};
+      variable_list from, by, to;
+      for (int i = 0; i < 3; ++i)
+        if (out[i].requires_grad()) { from.push_back(out[i]); by.push_back(grads[i]); }
+      for (const at::Tensor& t : of)
+        if (t.requires_grad()) to.push_back(t);
+      const auto got = torch::autograd::grad(from, to, by, true, true, true);
+      variable_list r(8);
+      for (int i = 0, at = 0; i < 3; ++i)
+        if (of[i].requires_grad()) r[i] = got[at++];
+      return r;
+    }
+    auto r = norm_rope_bwd(grads[0], grads[1], grads[2], s[0], s[1], s[2], s[3], maybe(s[4]), n[0], n[1], eps);
+    return {r[0], r[1], r[2], none, none, none, none, none};
+  }
+};
+
 bool direct(at::TensorList tensors) {
   for (const at::Tensor& t : tensors)
     if (!t.is_cuda() || !plain(t) || has_tangent(t)) return false;
@@ -189,6 +237,14 @@ Maybe native_fused_rope_attention(const at::Tensor& qkv, const at::Tensor& table
                                   int64_t D, bool causal, double scale, const Maybe& seqlens) {
   if (!direct({qkv})) return c10::nullopt;
   return FusedRopeAttention::apply(qkv, table, positions, Hq, Hkv, D, causal, scale, seqlens);
+}
+
+c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> native_norm_rope(const at::Tensor& qkv, const at::Tensor& wq, const at::Tensor& wk,
+                                                                               const at::Tensor& table, const Maybe& positions, int64_t Hq,
+                                                                               int64_t Hkv, double eps) {
+  if (!direct({qkv, wq, wk})) return c10::nullopt;
+  auto r = NormRope::apply(qkv, wq, wk, table, positions, Hq, Hkv, eps);
+  return std::make_tuple(r[0], r[1], r[2]);
 }
 
 }  // namespace cai
