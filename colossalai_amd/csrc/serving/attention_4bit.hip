@@ -1,0 +1,468 @@
+// Attention of a ragged step's tokens over a paged cache in 4 bits (cache_4bit.h), bfloat16 queries.
+//
+//   p_j = exp(scale q . k_j) over the keys j that the token sees,  out = sum p_j v_j / sum p_j
+//
+// A block takes 16 RT rows, the query heads of one key head for one or several tokens, and a part of their keys; its waves take steps of 32 keys
+// in turn and meet in LDS at the end. A wave works alone, on registers: codes come in one 16-byte load a tile of 16 tokens, become
+// bfloat16 by the conversion that takes two codes and their scale, and feed
+//   S^T = K Q^T (A = 16 tokens of keys, B = 16 rows of queries: a row is a lane's column, a lane has four tokens of a tile),
+//   O^T = V^T P^T (A = 16 channels of values, B = the weights where they were born: the tokens of a lane are the same in both).
+// One pass over the keys with a running reference and sum a row; a row's weights may pass its reference by 2^8 before sums are scaled anew.
+// Weights are rounded to bfloat16 for the product, their sum is that of the float32 ones. What no row sees is taken out of the values too:
+// its scale is set to 0, so that nothing behind a sequence's end shows.
+#include "cache_4bit.h"
+
+#include <c10/core/DeviceGuard.h>
+
+#include <algorithm>
+
+namespace cai {
+namespace serving {
+namespace {
+
+constexpr int STEP = 2 * TILE, WAVES4 = 4;
+constexpr float LOG2E4 = 1.4426950408889634f, SLACK = 8.0f;   // a weight may be up to 2^SLACK
+
+struct Attend {
+  const bf16s* q;
+  long q_stride, pages, page_stride;
+  const unsigned char *kpool, *vpool;
+  const int *tables, *tiles, *tok_seq, *positions;
+  bf16s* out;
+  float* parts;
+  int width, H, G, head_bytes, page_shift, window, splits, group, subs;
+  float scale;
+};
+
+// A step's codes and scales as they come.
+template <int D>
+struct Raw {
+  static constexpr int W = D / 32;   // 32-bit words of a lane's channels of a tile, keys or values
+  unsigned int k[2][W], v[2][W], ks[2], vs[2];
+  bool bad[2];
+};
+
+template <int W>
+DEV_INLINE void load_words(unsigned int (&w)[W], const unsigned char* p) {
+  if constexpr (W == 2) {
+    const uint2 t = *reinterpret_cast<const uint2*>(p);
+    w[0] = t.x; w[1] = t.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      const uint4 t = *reinterpret_cast<const uint4*>(p + 4 * i);
+      w[i] = t.x; w[i + 1] = t.y; w[i + 2] = t.z; w[i + 3] = t.w;
+    }
+  }
+}
+
+typedef unsigned int uint4v __attribute__((ext_vector_type(4)));
+DEV_INLINE bf16x8_v frag(unsigned int a, unsigned int b, unsigned int c, unsigned int d) {
+  return __builtin_bit_cast(bf16x8_v, uint4v{a, b, c, d});
+}
+DEV_INLINE unsigned int two_bf16(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned int, __builtin_convertvector((f2{a, b}), bf16x2));
+}
+template <int B>
+DEV_INLINE unsigned int number_pair(const unsigned int* words, float scale) { return two_numbers<B & 3>(words[B >> 2], scale); }
+
+// numbers of byte B of four tokens' values as fragments' words: tokens (0, 1) and (2, 3) of the byte's lower and upper channel
+template <int D, int B>
+DEV_INLINE void value_words(const unsigned int* w, const float* scale, unsigned int (&lo)[2], unsigned int (&hi)[2]) {
+  constexpr int S = D / 32;   // bytes of a token
+  const unsigned int t0 = number_pair<B>(w, scale[0]), t1 = number_pair<S + B>(w, scale[1]), t2 = number_pair<2 * S + B>(w, scale[2]),
+                     t3 = number_pair<3 * S + B>(w, scale[3]);
+  lo[0] = __builtin_amdgcn_perm(t1, t0, 0x05040100u);
+  hi[0] = __builtin_amdgcn_perm(t1, t0, 0x07060302u);
+  lo[1] = __builtin_amdgcn_perm(t3, t2, 0x05040100u);
+  hi[1] = __builtin_amdgcn_perm(t3, t2, 0x07060302u);
+}
+
+template <int N, typename F>
+DEV_INLINE void unrolled(F f) {
+  [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, N>());
+}
+
+template <int D, int RT>
+__global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
+  constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;   // rows, products of a tile's scores, tiles of channels
+  __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
+  float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int split = (int)(blockIdx.x % a.splits);
+  const long unit = blockIdx.x / a.splits;
+  const int g = (int)(unit % a.G), sub = (int)(unit / a.G % a.subs);
+  const long tile = unit / a.G / a.subs;
+  int seq, t0, t1;
+  if (a.tiles != nullptr) {
+    seq = a.tiles[tile * 4];
+    t0 = a.tiles[tile * 4 + 1];
+    t1 = a.tiles[tile * 4 + 2];
+  } else {
+    seq = a.tok_seq[tile];
+    t0 = (int)tile;
+    t1 = t0 + 1;
+  }
+  const int per_token = min(a.group, R);
+  const int p0 = a.positions[t0], p1 = a.positions[t1 - 1];
+  const int first = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
+
+  // rows: queries, positions, places
+  bf16x8_v q[RT][KF];
+  int pos[RT], tok[RT], head[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = rt * 16 + n, in = sub * R + r % per_token;
+    tok[rt] = t0 + r / per_token;
+    const bool real = tok[rt] < t1 && in < a.group;
+    head[rt] = real ? g * a.group + in : -1;
+    pos[rt] = real ? a.positions[tok[rt]] : p1;
+    const bf16s* from = a.q + (real ? tok[rt] : t0) * a.q_stride + (long)(real ? head[rt] : g * a.group) * D + kg * (D / 4);
+#pragma unroll
+    for (int f = 0; f < KF; ++f) q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
+  }
+
+  const int begin = first / STEP, steps = p1 / STEP + 1 - begin, share = (steps + a.splits - 1) / a.splits;
+  const int from = begin + split * share, to = min(begin + steps, from + share);
+  const int* table = a.tables + (long)seq * a.width;
+  const float scale = a.scale * LOG2E4;
+
+  auto load = [&](Raw<D>& w, int step) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = min(step * STEP + h * TILE, p1);   // a tile behind the end is its last one again: hidden by its places
+      const int page = table[at >> a.page_shift];
+      w.bad[h] = (unsigned)page >= (unsigned long)a.pages;
+      const long base = (long)(w.bad[h] ? 0 : page) * a.page_stride + (long)g * a.head_bytes +
+                        (long)((at & ((1 << a.page_shift) - 1)) / TILE) * Tile4<D>::BYTES;
+      const unsigned char *kt = a.kpool + base, *vt = a.vpool + base;
+      load_words(w.k[h], kt + n * (D / 2) + kg * (D / 8));
+      if constexpr (D == 256) w.ks[h] = *reinterpret_cast<const unsigned short*>(kt + Tile4<D>::key_scale(n, 2 * kg));
+      else w.ks[h] = kt[Tile4<D>::key_scale(n, D == 128 ? kg : kg >> 1)];
+      load_words(w.v[h], vt + (kg * 16 + n) * (D / 8));
+      w.vs[h] = *reinterpret_cast<const unsigned int*>(vt + Tile4<D>::value_scale(kg * 4, n * (D / 16) / 32));
+    }
+  };
+
+  f32x4 o[RT][VF];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    m[rt] = -INFINITY;
+    l[rt] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < VF; ++f) o[rt][f] = f32x4{0, 0, 0, 0};
+  }
+
+  auto compute = [&](const Raw<D>& w, int step) {
+    const int j = step * STEP;
+    // whether some row does not see some key of the step
+    const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][h] = f32x4{0, 0, 0, 0};
+      const float ks = scale_of(w.ks[h] & 255u), ks2 = scale_of(D == 256 ? w.ks[h] >> 8 : w.ks[h] & 255u);
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const float u = D == 256 && f >= 4 ? ks2 : ks;
+        const unsigned int x = w.k[h][f];
+        const bf16x8_v k = frag(two_numbers<0>(x, u), two_numbers<1>(x, u), two_numbers<2>(x, u), two_numbers<3>(x, u));
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[rt][f], s[rt][h], 0, 0, 0);
+      }
+    }
+    unsigned int vs[2] = {w.vs[0], w.vs[1]};
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[rt][h] *= scale;
+    if (edge) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = j + h * TILE + kg * 4 + i;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const bool seen = key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window);
+            s[rt][h][i] = !seen ? -INFINITY : w.bad[h] ? __builtin_nanf("") : s[rt][h][i];
+          }
+          if (key > p1 || (a.window > 0 && p0 - key >= a.window)) vs[h] &= ~(255u << (8 * i));
+        }
+      // a value that is not finite goes to the rows that see it through their weights: a weight of 0 would not hide it from the others
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned long long odd = __ballot(((vs[h] >> (8 * i)) & 255u) == 255u);
+          if (odd == 0) continue;
+          if ((odd >> (16 * kg)) & 0xffffu) {
+            const int key = j + h * TILE + kg * 4 + i;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              if (key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window)) s[rt][h][i] = __builtin_nanf("");
+            vs[h] &= ~(255u << (8 * i));
+          }
+        }
+    }
+    bf16x8_v p[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__any(top > m[rt] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
+        const float next = fmaxf(m[rt], top), fall = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - next);
+        m[rt] = next;
+        l[rt] *= fall;
+#pragma unroll
+        for (int f = 0; f < VF; ++f) o[rt][f] *= fall;
+      }
+      const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
+      float e[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[h * 4 + i] = __builtin_amdgcn_exp2f(s[rt][h][i] - ref);
+          l[rt] += e[h * 4 + i];
+        }
+      p[rt] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
+    }
+    float su[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) su[h][i] = scale_of((vs[h] >> (8 * i)) & 255u);
+    unrolled<D / 32>([&](auto byte) {
+      constexpr int B = decltype(byte)::value;
+      unsigned int lo0[2], hi0[2], lo1[2], hi1[2];
+      value_words<D, B>(w.v[0], su[0], lo0, hi0);
+      value_words<D, B>(w.v[1], su[1], lo1, hi1);
+      const bf16x8_v lo = frag(lo0[0], lo0[1], lo1[0], lo1[1]), hi = frag(hi0[0], hi0[1], hi1[0], hi1[1]);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt], o[rt][2 * B], 0, 0, 0);
+        o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt], o[rt][2 * B + 1], 0, 0, 0);
+      }
+    });
+  };
+
+  // the next step's codes are on their way while a step is worked on
+  int step = from + wid;
+  if (step < to) {
+    Raw<D> now, next;
+    load(now, step);
+    for (; step < to; step += WAVES4) {
+      if (step + WAVES4 < to) load(next, step + WAVES4);
+      compute(now, step);
+      now = next;
+    }
+  }
+
+  // the waves' states meet: a common reference, then sums in pairs
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += __shfl_xor(l[rt], 16);
+    l[rt] += __shfl_xor(l[rt], 32);
+    if (kg == 0) states[wid][rt * 16 + n] = float2v{m[rt], l[rt]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES4; ++w) top = fmaxf(top, states[w][rt * 16 + n][0]);
+#pragma unroll
+    for (int w = 0; w < WAVES4; ++w) {
+      const float2v x = states[w][rt * 16 + n];   // without a reference the sum is 0, or NaN, which stays
+      sum += x[0] == -INFINITY ? x[1] : x[1] * __builtin_amdgcn_exp2f(x[0] - top);
+    }
+    const float mine = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
+#pragma unroll
+    for (int f = 0; f < VF; ++f) o[rt][f] *= mine;
+    m[rt] = top;
+    l[rt] = sum;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int live = WAVES4 / 2; live > 0; live >>= 1) {
+    if (wid >= live && wid < 2 * live) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int f = 0; f < VF; ++f) lds[wid - live][rt * VF + f][lane] = o[rt][f];
+    }
+    __syncthreads();
+    if (wid < live) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int f = 0; f < VF; ++f) o[rt][f] += lds[wid][rt * VF + f][lane];
+    }
+    __syncthreads();
+  }
+  if (wid != 0) return;
+  if (a.splits == 1) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (head[rt] < 0) continue;
+      const float inv = 1.0f / l[rt];
+      bf16s* to_row = a.out + ((long)tok[rt] * a.H + head[rt]) * D;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        unsigned int w[VF / 2];
+#pragma unroll
+        for (int f = 0; f < VF; f += 2) w[f / 2] = two_bf16(o[rt][f][i] * inv, o[rt][f + 1][i] * inv);
+        unsigned int* to_ch = reinterpret_cast<unsigned int*>(to_row + (kg * 4 + i) * VF);
+#pragma unroll
+        for (int f = 0; f < VF / 2; f += 2) *reinterpret_cast<uint2*>(to_ch + f) = make_uint2(w[f], w[f + 1]);
+      }
+    }
+    return;
+  }
+  // a part: rows' sums, then their references and weights
+  float* part = a.parts + (unit * a.splits + split) * (R * (D + 2L));
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int f = 0; f < VF; f += 4)
+        *reinterpret_cast<float4v*>(part + (rt * 16 + n) * D + (kg * 4 + i) * VF + f) = float4v{o[rt][f][i], o[rt][f + 1][i], o[rt][f + 2][i], o[rt][f + 3][i]};
+    if (kg == 0) *reinterpret_cast<float2v*>(part + (long)R * D + (rt * 16 + n) * 2) = float2v{m[rt], l[rt]};
+  }
+}
+
+// Puts the parts of a unit's rows together: eight channels a thread.
+template <int D, int RT>
+__global__ __launch_bounds__(256) void attention_4bit_merge_kernel(Attend a, long units) {
+  constexpr int R = 16 * RT;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(i % (D / 8)) * 8, r = (int)(i / (D / 8) % R);
+  const long unit = i / (D / 8) / R;
+  if (unit >= units) return;
+  const int g = (int)(unit % a.G), sub = (int)(unit / a.G % a.subs);
+  const long tile = unit / a.G / a.subs;
+  const int t0 = a.tiles != nullptr ? a.tiles[tile * 4 + 1] : (int)tile, t1 = a.tiles != nullptr ? a.tiles[tile * 4 + 2] : t0 + 1;
+  const int per_token = min(a.group, R), tok = t0 + r / per_token, in = sub * R + r % per_token;
+  if (tok >= t1 || in >= a.group) return;
+  const float* part = a.parts + unit * a.splits * (R * (D + 2L));
+  float top = -INFINITY, sum = 0.0f, o[8] = {};
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[s * (R * (D + 2L)) + (long)R * D + r * 2]);
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = part + s * (R * (D + 2L));
+    const float m = p[(long)R * D + r * 2], l = p[(long)R * D + r * 2 + 1];
+    if (m == -INFINITY && l == 0.0f) continue;   // nothing seen; a sum of NaN stays
+    const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    sum += w * l;
+    float x[8];
+    load8(p + r * D + c, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += w * x[e];
+  }
+  const float inv = 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] *= inv;
+  store8(a.out + ((long)tok * a.H + g * a.group + in) * D + c, o);
+}
+
+template <int D, int RT>
+void launch(Attend a, long tiles, int64_t longest, const at::Tensor& like) {
+  a.subs = (a.group + 16 * RT - 1) / (16 * RT);
+  const long units = tiles * a.G * a.subs, steps = (longest + STEP - 1) / STEP + 1;
+  // enough blocks for the chip, as long as a wave has two steps
+  a.splits = (int)std::max<long>(1, std::min<long>({64, 1024 / units, steps / (2 * WAVES4)}));
+  at::Tensor parts;
+  if (a.splits > 1) {
+    parts = at::empty({units * a.splits * 16 * RT * (D + 2)}, like.options().dtype(at::kFloat));
+    a.parts = parts.data_ptr<float>();
+  }
+  hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(units * a.splits)), dim3(64 * WAVES4), 0, stream(), a);
+  HIP_CHECK_LAST();
+  if (a.splits > 1) {
+    hipLaunchKernelGGL((attention_4bit_merge_kernel<D, RT>), dim3((unsigned)((units * 16 * RT * (D / 8) + 255) / 256)), dim3(256), 0, stream(), a,
+                       units);
+    HIP_CHECK_LAST();
+  }
+}
+
+}  // namespace
+
+// `tiles` [K, 4]: (sequence, first token, end token, 0), the first `few` of them with at most 16 rows, the others with at most 16 * `row_tiles`;
+// without, every token is a tile. `longest_*`: the most keys that a tile of the kind sees.
+at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor tok_seq,
+                                at::Tensor positions, c10::optional<at::Tensor> tiles, int64_t few, int64_t row_tiles, int64_t longest_few,
+                                int64_t longest_many, double scale, int64_t window, int64_t page_size) {
+  const char* who = "paged_attention_4bit: ";
+  TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 3 && is_bf16(q_in), who, "q must be bfloat16 [N, H, D]");
+  const c10::DeviceGuard guard(q_in.device());
+  const int64_t N = q_in.size(0), H = q_in.size(1), D = q_in.size(2);
+  TORCH_CHECK(D == 64 || D == 128 || D == 256, who, "heads of 64, 128 or 256 channels, got ", D);
+  TORCH_CHECK(page_size_of(kpool, D) == page_size && page_size_of(vpool, D) == page_size && kpool.sizes() == vpool.sizes() && kpool.size(0) > 0, who,
+              "pools must be contiguous uint8 [pages, heads, page size * 17 * D / 32] of the batch's page size ", page_size);
+  const int64_t G = kpool.size(1);
+  TORCH_CHECK(G > 0 && H % G == 0, who, H, " query heads cannot share ", G, " key heads");
+  check_i32(block_tables, "block_tables");
+  check_i32(tok_seq, "tok_seq");
+  check_i32(positions, "positions");
+  TORCH_CHECK(block_tables.dim() == 2 && tok_seq.numel() == N && positions.numel() == N, who, "batch of other tokens");
+  for (const at::Tensor& t : {kpool, vpool, block_tables, tok_seq, positions, tiles.value_or(q_in)})
+    TORCH_CHECK(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
+  const bool fits = q_in.stride(2) == 1 && q_in.stride(1) == D && q_in.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
+  const at::Tensor q = fits ? q_in : q_in.clone(at::MemoryFormat::Contiguous), out = at::empty({N, H, D}, q.options());
+  if (N == 0) return out;
+  Attend a;
+  a.q = ptr<bf16s>(q);
+  a.q_stride = q.stride(0);
+  a.pages = kpool.size(0);
+  a.page_stride = kpool.size(1) * kpool.size(2);
+  a.head_bytes = (int)kpool.size(2);
+  a.kpool = kpool.data_ptr<uint8_t>();
+  a.vpool = vpool.data_ptr<uint8_t>();
+  a.tables = block_tables.data_ptr<int>();
+  a.tok_seq = tok_seq.data_ptr<int>();
+  a.positions = positions.data_ptr<int>();
+  a.out = ptr<bf16s>(out);
+  a.width = (int)block_tables.size(1);
+  a.H = (int)H;
+  a.G = (int)G;
+  a.group = (int)(H / G);
+  a.page_shift = 0;
+  while ((1L << a.page_shift) < page_size) ++a.page_shift;
+  a.window = (int)std::min<int64_t>(window, 1L << 30);
+  a.scale = (float)scale;
+  auto run = [&](auto size) {
+    constexpr int DD = decltype(size)::value;
+    if (!tiles.has_value()) {
+      a.tiles = nullptr;
+      launch<DD, 1>(a, N, longest_few, q);
+      return;
+    }
+    check_i32(*tiles, "tiles");
+    TORCH_CHECK(tiles->dim() == 2 && tiles->size(1) == 4 && few >= 0 && few <= tiles->size(0) && (row_tiles == 2 || row_tiles == 4), who, "tiles");
+    const long many = tiles->size(0) - few;
+    a.tiles = tiles->data_ptr<int>();
+    if (few > 0) launch<DD, 1>(a, few, longest_few, q);
+    a.tiles += 4 * few;
+    if (many > 0) {
+      if (row_tiles == 2) launch<DD, 2>(a, many, longest_many, q);
+      else if constexpr (DD <= 128) launch<DD, 4>(a, many, longest_many, q);
+      else TORCH_CHECK(false, who, "64 rows a tile for heads of up to 128 channels");
+    }
+  };
+  if (D == 64) run(std::integral_constant<int, 64>());
+  else if (D == 128) run(std::integral_constant<int, 128>());
+  else run(std::integral_constant<int, 256>());
+  return out;
+}
+
+}  // namespace serving
+}  // namespace cai

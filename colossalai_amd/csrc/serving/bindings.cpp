@@ -77,6 +77,12 @@ void rotate_qk_write(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor freqs,
                      at::Tensor vpool, at::Tensor rows);
 void latent_kv_write(at::Tensor dkv, at::Tensor norm_w, double eps, at::Tensor freqs, at::Tensor positions,
                      at::Tensor pool, at::Tensor rows);
+at::Tensor paged_kv_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor kpool, at::Tensor vpool, at::Tensor rows, at::Tensor positions,
+                           at::Tensor table, c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, double eps);
+std::vector<at::Tensor> kv4_read(at::Tensor kpool, at::Tensor vpool, at::Tensor rows, int64_t D);
+at::Tensor paged_attention_4bit(at::Tensor q, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor tok_seq,
+                                at::Tensor positions, c10::optional<at::Tensor> tiles, int64_t few, int64_t row_tiles, int64_t longest_few,
+                                int64_t longest_many, double scale, int64_t window, int64_t page_size);
 std::vector<at::Tensor> expert_sort(at::Tensor ids, int64_t num_experts);
 at::Tensor expert_grouped_gemm(at::Tensor a, c10::optional<at::Tensor> a_rows, at::Tensor w, at::Tensor offsets,
                                int64_t rows, bool relu_squared);
@@ -127,6 +133,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rotate_qk_write", &s::rotate_qk_write,
         "rotary positions on neighbouring pairs: queries in place, keys into pool rows, values into pool rows");
   m.def("latent_kv_write", &s::latent_kv_write, "latent row: RMS norm + pair rotation + scatter into pool rows");
+  m.def("paged_kv_append", &s::paged_kv_append,
+        "norm and rotation of new queries and keys; keys and values into pool rows, in their type or in 4 bits");
+  m.def("kv4_read", &s::kv4_read, "the numbers of a 4-bit cache's rows");
+  m.def("paged_attention_4bit", &s::paged_attention_4bit, "ragged paged attention over a 4-bit cache");
   m.def("expert_ffn_gemv", &s::expert_ffn_gemv, "chosen experts' feed-forward of a small step, matrix-vector kernels");
   m.def("expert_sort", &s::expert_sort, "stable sort of (token, expert) pairs by expert: offsets, source tokens, inverse");
   m.def("expert_grouped_gemm", &s::expert_grouped_gemm,

@@ -1,6 +1,7 @@
 from ._kernels import has_kernels, kernels, use_hip
 from .grouped_gemm import grouped_gemm
 from .attention import attention_ref, flash_attention, flash_attention_varlen, fused_rope_attention, seqlens_from_attention_mask
+from .cache_4bit import kv4_pool, kv4_read, paged_attention_4bit, paged_kv_append
 from .layernorm import layer_norm
 from .norm_rope import qkv_norm_rope
 from .norm import fused_add_rms_norm, rms_norm, rms_norm_ref
@@ -20,6 +21,10 @@ __all__ = [
     "rms_norm",
     "layer_norm",
     "qkv_norm_rope",
+    "kv4_pool",
+    "kv4_read",
+    "paged_attention_4bit",
+    "paged_kv_append",
     "fused_add_rms_norm",
     "rms_norm_ref",
     "apply_rope",

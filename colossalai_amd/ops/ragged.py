@@ -80,6 +80,7 @@ class RaggedBatch:
     _tiles: Optional[tuple] = None  # memo of tile_counts()
     _singles: Optional[tuple] = None  # memo of single_tokens()
     _even: Optional[dict] = None  # memo of key_lengths(), by window and fewest
+    _rows: Optional[dict] = None  # memo of query_tiles(), by group, most and window
 
     @property
     def num_seqs(self) -> int:
@@ -137,6 +138,34 @@ class RaggedBatch:
                 most = max(most, min(hi, window) if window > 0 else hi)
             self._even[window, fewest] = (total / (tiles * most), int(most)) if tiles else (0.5, 0)
         return self._even[window, fewest]
+
+    def query_tiles(self, group: int, most: int, window: int = 0):
+        """For attention that takes the `group` query heads of a key head for a few tokens as the rows of a tile:
+        ``(tiles, few, row_tiles, longest_few, longest_many)``. ``tiles`` [K, 4] int32 = (sequence, first token, end token, 0): first `few` of
+        sequences whose new tokens are at most 16 rows, or one token, then those of the others, 16 * `row_tiles` rows each (2, or up to `most`),
+        the ones with the most keys first; None where every sequence brings one token. ``longest_*``: the most keys that a tile of the kind
+        sees. Built once per step, shared by its layers."""
+        if self._rows is None:
+            self._rows = {}
+        if (group, most, window) not in self._rows:
+            spans = list(zip(range(self.num_seqs), self.cu_host, self.cu_host[1:], self.start_host))
+            seen = lambda first, end: min(end, window + end - first - 1) if window > 0 else end  # noqa: E731
+            few, many, row_tiles = [], [], 2
+            if any((b - a) * group > 32 and b - a > 1 for _, a, b, _ in spans):
+                row_tiles = most
+            for i, a, b, s in spans:
+                short = b - a == 1 or (b - a) * group <= 16
+                per = max(1, (16 if short else 16 * row_tiles) // group)
+                for t in range(a, b, per):
+                    end = min(t + per, b)
+                    (few if short else many).append((seen(s + t - a, s + end - a), i, t, end))
+            many.sort(key=lambda x: -x[0])
+            longest = [max((x[0] for x in part), default=0) for part in (few, many)]
+            tiles = None
+            if self.num_tokens != self.num_seqs:
+                tiles = to_device([v for x in few + many for v in (*x[1:], 0)], torch.int32, self.cu.device, self.ordered).view(-1, 4)
+            self._rows[group, most, window] = (tiles, len(few), row_tiles, *longest)
+        return self._rows[group, most, window]
 
     @property
     def num_tiles32(self) -> int:
