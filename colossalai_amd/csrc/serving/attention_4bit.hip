@@ -8,7 +8,7 @@
 //   S^T = K Q^T (A = 16 tokens of keys, B = 16 rows of queries: a row is a lane's column, a lane has four tokens of a tile),
 //   O^T = V^T P^T (A = 16 channels of values, B = the weights where they were born: the tokens of a lane are the same in both).
 // One pass over the keys with a running reference and sum a row; a row's weights may pass its reference by 2^8 before sums are scaled anew.
-// Weights are rounded to bfloat16 for the product, their sum is that of the float32 ones. What no row sees is taken out of the values too:
+// Weights are rounded to bfloat16 for the product, of tiles of 16 rows in two pieces, 16 of their 24 bits; their sum is that of the float32 ones. What no row sees is taken out of the values too:
 // its scale is set to 0, so that nothing behind a sequence's end shows.
 #include "cache_4bit.h"
 
@@ -27,10 +27,10 @@ struct Attend {
   const bf16s* q;
   long q_stride, pages, page_stride;
   const unsigned char *kpool, *vpool;
-  const int *tables, *tiles, *tok_seq, *positions;
+  const int *tables, *items, *joins, *positions;
   bf16s* out;
   float* parts;
-  int width, H, G, head_bytes, page_shift, window, splits, group, subs;
+  int width, H, G, head_bytes, page_shift, window, group, subs;
   float scale;
 };
 
@@ -85,28 +85,16 @@ DEV_INLINE void unrolled(F f) {
 }
 
 template <int D, int RT>
-__global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
+__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attention_4bit_kernel(Attend a) {
   constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;   // rows, products of a tile's scores, tiles of channels
   __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
   float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int split = (int)(blockIdx.x % a.splits);
-  const long unit = blockIdx.x / a.splits;
-  const int g = (int)(unit % a.G), sub = (int)(unit / a.G % a.subs);
-  const long tile = unit / a.G / a.subs;
-  int seq, t0, t1;
-  if (a.tiles != nullptr) {
-    seq = a.tiles[tile * 4];
-    t0 = a.tiles[tile * 4 + 1];
-    t1 = a.tiles[tile * 4 + 2];
-  } else {
-    seq = a.tok_seq[tile];
-    t0 = (int)tile;
-    t1 = t0 + 1;
-  }
+  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
+  const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
+  const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
   const int per_token = min(a.group, R);
   const int p0 = a.positions[t0], p1 = a.positions[t1 - 1];
-  const int first = a.window > 0 ? max(0, p0 - a.window + 1) : 0;
 
   // rows: queries, positions, places
   bf16x8_v q[RT][KF];
@@ -123,8 +111,6 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
     for (int f = 0; f < KF; ++f) q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
   }
 
-  const int begin = first / STEP, steps = p1 / STEP + 1 - begin, share = (steps + a.splits - 1) / a.splits;
-  const int from = begin + split * share, to = min(begin + steps, from + share);
   const int* table = a.tables + (long)seq * a.width;
   const float scale = a.scale * LOG2E4;
 
@@ -208,7 +194,7 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
           }
         }
     }
-    bf16x8_v p[RT];
+    bf16x8_v p[RT], rest[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top = -INFINITY;
@@ -234,7 +220,13 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
           e[h * 4 + i] = __builtin_amdgcn_exp2f(s[rt][h][i] - ref);
           l[rt] += e[h * 4 + i];
         }
-      p[rt] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
+      const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
+      p[rt] = __builtin_bit_cast(bf16x8_v, w);
+      if constexpr (RT == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        rest[rt] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
+      }
     }
     float su[2][4];
 #pragma unroll
@@ -251,6 +243,10 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
       for (int rt = 0; rt < RT; ++rt) {
         o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt], o[rt][2 * B], 0, 0, 0);
         o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt], o[rt][2 * B + 1], 0, 0, 0);
+        if constexpr (RT == 1) {
+          o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt], o[rt][2 * B], 0, 0, 0);
+          o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt], o[rt][2 * B + 1], 0, 0, 0);
+        }
       }
     });
   };
@@ -310,7 +306,7 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
     __syncthreads();
   }
   if (wid != 0) return;
-  if (a.splits == 1) {
+  if (slot < 0) {   // the only part
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (head[rt] < 0) continue;
@@ -329,9 +325,10 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
     return;
   }
   // a part: rows' sums, then their references and weights
-  float* part = a.parts + (unit * a.splits + split) * (R * (D + 2L));
+  float* part = a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L));
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
+    if (head[rt] < 0) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -341,27 +338,28 @@ __global__ __launch_bounds__(64 * WAVES4) void attention_4bit_kernel(Attend a) {
   }
 }
 
-// Puts the parts of a unit's rows together: eight channels a thread.
+// Puts the parts of a tile's rows together: eight channels a thread.
 template <int D, int RT>
-__global__ __launch_bounds__(256) void attention_4bit_merge_kernel(Attend a, long units) {
+__global__ __launch_bounds__(256) void attention_4bit_join_kernel(Attend a, long units) {
   constexpr int R = 16 * RT;
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   const int c = (int)(i % (D / 8)) * 8, r = (int)(i / (D / 8) % R);
   const long unit = i / (D / 8) / R;
   if (unit >= units) return;
   const int g = (int)(unit % a.G), sub = (int)(unit / a.G % a.subs);
-  const long tile = unit / a.G / a.subs;
-  const int t0 = a.tiles != nullptr ? a.tiles[tile * 4 + 1] : (int)tile, t1 = a.tiles != nullptr ? a.tiles[tile * 4 + 2] : t0 + 1;
+  const int* join = a.joins + unit / a.G / a.subs * 4;
+  const int t0 = join[0], t1 = join[1], count = join[3];
   const int per_token = min(a.group, R), tok = t0 + r / per_token, in = sub * R + r % per_token;
   if (tok >= t1 || in >= a.group) return;
-  const float* part = a.parts + unit * a.splits * (R * (D + 2L));
+  const float* part = a.parts + (((long)join[2] * a.subs + sub) * a.G + g) * (R * (D + 2L));
+  const long next = (long)a.subs * a.G * (R * (D + 2L));
   float top = -INFINITY, sum = 0.0f, o[8] = {};
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[s * (R * (D + 2L)) + (long)R * D + r * 2]);
-  for (int s = 0; s < a.splits; ++s) {
-    const float* p = part + s * (R * (D + 2L));
+  for (int s = 0; s < count; ++s) top = fmaxf(top, part[s * next + (long)R * D + r * 2]);
+#pragma unroll 4
+  for (int s = 0; s < count; ++s) {
+    const float* p = part + s * next;
     const float m = p[(long)R * D + r * 2], l = p[(long)R * D + r * 2 + 1];
-    if (m == -INFINITY && l == 0.0f) continue;   // nothing seen; a sum of NaN stays
-    const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+    const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);   // without a reference all is 0, or NaN, which stays
     sum += w * l;
     float x[8];
     load8(p + r * D + c, x);
@@ -375,32 +373,30 @@ __global__ __launch_bounds__(256) void attention_4bit_merge_kernel(Attend a, lon
 }
 
 template <int D, int RT>
-void launch(Attend a, long tiles, int64_t longest, const at::Tensor& like) {
+void launch(Attend a, long items, long slots, long joins, const at::Tensor& like) {
   a.subs = (a.group + 16 * RT - 1) / (16 * RT);
-  const long units = tiles * a.G * a.subs, steps = (longest + STEP - 1) / STEP + 1;
-  // enough blocks for the chip, as long as a wave has two steps
-  a.splits = (int)std::max<long>(1, std::min<long>({64, 1024 / units, steps / (2 * WAVES4)}));
+  const long heads = (long)a.G * a.subs;
   at::Tensor parts;
-  if (a.splits > 1) {
-    parts = at::empty({units * a.splits * 16 * RT * (D + 2)}, like.options().dtype(at::kFloat));
+  if (joins > 0) {
+    parts = at::empty({slots * heads * 16 * RT * (D + 2)}, like.options().dtype(at::kFloat));
     a.parts = parts.data_ptr<float>();
   }
-  hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(units * a.splits)), dim3(64 * WAVES4), 0, stream(), a);
+  hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(items * heads)), dim3(64 * WAVES4), 0, stream(), a);
   HIP_CHECK_LAST();
-  if (a.splits > 1) {
-    hipLaunchKernelGGL((attention_4bit_merge_kernel<D, RT>), dim3((unsigned)((units * 16 * RT * (D / 8) + 255) / 256)), dim3(256), 0, stream(), a,
-                       units);
+  if (joins > 0) {
+    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)((joins * heads * 16 * RT * (D / 8) + 255) / 256)), dim3(256), 0, stream(),
+                       a, joins * heads);
     HIP_CHECK_LAST();
   }
 }
 
 }  // namespace
 
-// `tiles` [K, 4]: (sequence, first token, end token, 0), the first `few` of them with at most 16 rows, the others with at most 16 * `row_tiles`;
-// without, every token is a tile. `longest_*`: the most keys that a tile of the kind sees.
-at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor tok_seq,
-                                at::Tensor positions, c10::optional<at::Tensor> tiles, int64_t few, int64_t row_tiles, int64_t longest_few,
-                                int64_t longest_many, double scale, int64_t window, int64_t page_size) {
+// `plan`: of the tiles with at most 16 rows, then of those with at most 32, what a block does, (sequence, first token, end token, first step,
+// end step, part or -1) for each, then the tiles that have parts, (first token, end token, first part, parts). `sizes`: of each kind the numbers of
+// both, and of parts.
+at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions,
+                                at::Tensor plan, std::vector<int64_t> sizes, double scale, int64_t window, int64_t page_size) {
   const char* who = "paged_attention_4bit: ";
   TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 3 && is_bf16(q_in), who, "q must be bfloat16 [N, H, D]");
   const c10::DeviceGuard guard(q_in.device());
@@ -411,10 +407,11 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   const int64_t G = kpool.size(1);
   TORCH_CHECK(G > 0 && H % G == 0, who, H, " query heads cannot share ", G, " key heads");
   check_i32(block_tables, "block_tables");
-  check_i32(tok_seq, "tok_seq");
+  check_i32(plan, "plan");
   check_i32(positions, "positions");
-  TORCH_CHECK(block_tables.dim() == 2 && tok_seq.numel() == N && positions.numel() == N, who, "batch of other tokens");
-  for (const at::Tensor& t : {kpool, vpool, block_tables, tok_seq, positions, tiles.value_or(q_in)})
+  TORCH_CHECK(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 6 &&
+              plan.numel() == 6 * (sizes[0] + sizes[3]) + 4 * (sizes[1] + sizes[4]), who, "batch of other tokens");
+  for (const at::Tensor& t : {kpool, vpool, block_tables, positions, plan})
     TORCH_CHECK(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
   const bool fits = q_in.stride(2) == 1 && q_in.stride(1) == D && q_in.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
   const at::Tensor q = fits ? q_in : q_in.clone(at::MemoryFormat::Contiguous), out = at::empty({N, H, D}, q.options());
@@ -428,7 +425,6 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   a.kpool = kpool.data_ptr<uint8_t>();
   a.vpool = vpool.data_ptr<uint8_t>();
   a.tables = block_tables.data_ptr<int>();
-  a.tok_seq = tok_seq.data_ptr<int>();
   a.positions = positions.data_ptr<int>();
   a.out = ptr<bf16s>(out);
   a.width = (int)block_tables.size(1);
@@ -441,21 +437,15 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   a.scale = (float)scale;
   auto run = [&](auto size) {
     constexpr int DD = decltype(size)::value;
-    if (!tiles.has_value()) {
-      a.tiles = nullptr;
-      launch<DD, 1>(a, N, longest_few, q);
-      return;
-    }
-    check_i32(*tiles, "tiles");
-    TORCH_CHECK(tiles->dim() == 2 && tiles->size(1) == 4 && few >= 0 && few <= tiles->size(0) && (row_tiles == 2 || row_tiles == 4), who, "tiles");
-    const long many = tiles->size(0) - few;
-    a.tiles = tiles->data_ptr<int>();
-    if (few > 0) launch<DD, 1>(a, few, longest_few, q);
-    a.tiles += 4 * few;
-    if (many > 0) {
-      if (row_tiles == 2) launch<DD, 2>(a, many, longest_many, q);
-      else if constexpr (DD <= 128) launch<DD, 4>(a, many, longest_many, q);
-      else TORCH_CHECK(false, who, "64 rows a tile for heads of up to 128 channels");
+    const int* at = plan.data_ptr<int>();
+    for (int kind = 0; kind < 2; ++kind) {
+      const long items = sizes[3 * kind], joins = sizes[3 * kind + 1], slots = sizes[3 * kind + 2];
+      a.items = at;
+      a.joins = at + 6 * items;
+      at = a.joins + 4 * joins;
+      if (items == 0) continue;
+      if (kind == 0) launch<DD, 1>(a, items, slots, joins, q);
+      else launch<DD, 2>(a, items, slots, joins, q);
     }
   };
   if (D == 64) run(std::integral_constant<int, 64>());

@@ -80,9 +80,8 @@ void latent_kv_write(at::Tensor dkv, at::Tensor norm_w, double eps, at::Tensor f
 at::Tensor paged_kv_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor kpool, at::Tensor vpool, at::Tensor rows, at::Tensor positions,
                            at::Tensor table, c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, double eps);
 std::vector<at::Tensor> kv4_read(at::Tensor kpool, at::Tensor vpool, at::Tensor rows, int64_t D);
-at::Tensor paged_attention_4bit(at::Tensor q, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor tok_seq,
-                                at::Tensor positions, c10::optional<at::Tensor> tiles, int64_t few, int64_t row_tiles, int64_t longest_few,
-                                int64_t longest_many, double scale, int64_t window, int64_t page_size);
+at::Tensor paged_attention_4bit(at::Tensor q, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions, at::Tensor plan,
+                                std::vector<int64_t> sizes, double scale, int64_t window, int64_t page_size);
 std::vector<at::Tensor> expert_sort(at::Tensor ids, int64_t num_experts);
 at::Tensor expert_grouped_gemm(at::Tensor a, c10::optional<at::Tensor> a_rows, at::Tensor w, at::Tensor offsets,
                                int64_t rows, bool relu_squared);

@@ -225,6 +225,8 @@ def paged_attention_4bit(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tens
         return paged_attention_4bit_ref(q, kpool, vpool, batch, scale, window)
     if q.dtype != torch.bfloat16:
         raise ValueError(f"on a GPU the queries are bfloat16, got {q.dtype}")
-    tiles = batch.query_tiles(q.shape[1] // G, 4 if q.shape[2] <= 128 else 2, window)
-    return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.tok_seq, batch.positions, *tiles, float(scale),
-                                                  int(window), ps)
+    # what a chip of 256 CUs holds at once, by the kernel's registers
+    blocks = {64: (1024, 512), 128: (768, 512), 256: (512, 256)}[q.shape[2]]
+    subs = -(-(q.shape[1] // G) // 16)
+    plan, sizes = batch.row_plan(q.shape[1] // G, G * subs, window, blocks)
+    return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.positions, plan, sizes, float(scale), int(window), ps)

@@ -80,7 +80,7 @@ class RaggedBatch:
     _tiles: Optional[tuple] = None  # memo of tile_counts()
     _singles: Optional[tuple] = None  # memo of single_tokens()
     _even: Optional[dict] = None  # memo of key_lengths(), by window and fewest
-    _rows: Optional[dict] = None  # memo of query_tiles(), by group, most and window
+    _rows: Optional[dict] = None  # memo of row_plan(), by its arguments
 
     @property
     def num_seqs(self) -> int:
@@ -139,33 +139,59 @@ class RaggedBatch:
             self._even[window, fewest] = (total / (tiles * most), int(most)) if tiles else (0.5, 0)
         return self._even[window, fewest]
 
-    def query_tiles(self, group: int, most: int, window: int = 0):
-        """For attention that takes the `group` query heads of a key head for a few tokens as the rows of a tile:
-        ``(tiles, few, row_tiles, longest_few, longest_many)``. ``tiles`` [K, 4] int32 = (sequence, first token, end token, 0): first `few` of
-        sequences whose new tokens are at most 16 rows, or one token, then those of the others, 16 * `row_tiles` rows each (2, or up to `most`),
-        the ones with the most keys first; None where every sequence brings one token. ``longest_*``: the most keys that a tile of the kind
-        sees. Built once per step, shared by its layers."""
+    def row_plan(self, group: int, heads: int, window: int = 0, blocks: Sequence[int] = (1024, 512), step: int = 32, least: int = 8):
+        """The work of an attention kernel whose block takes a tile of rows (the `group` query heads of a key head for some tokens) and a part of
+        their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles have 16
+        rows where a sequence's new tokens are at most as many rows, or one token, else 32. A tile's keys are cut into even parts of at
+        least `least` steps, as many as the `blocks` that a chip holds at once (of tiles of 16 and of 32 rows) allow; `heads` blocks share a part.
+        Tiles with more keys come first. Built once per step and kind, shared by its layers."""
         if self._rows is None:
             self._rows = {}
-        if (group, most, window) not in self._rows:
-            spans = list(zip(range(self.num_seqs), self.cu_host, self.cu_host[1:], self.start_host))
-            seen = lambda first, end: min(end, window + end - first - 1) if window > 0 else end  # noqa: E731
-            few, many, row_tiles = [], [], 2
-            if any((b - a) * group > 32 and b - a > 1 for _, a, b, _ in spans):
-                row_tiles = most
-            for i, a, b, s in spans:
-                short = b - a == 1 or (b - a) * group <= 16
-                per = max(1, (16 if short else 16 * row_tiles) // group)
-                for t in range(a, b, per):
-                    end = min(t + per, b)
-                    (few if short else many).append((seen(s + t - a, s + end - a), i, t, end))
-            many.sort(key=lambda x: -x[0])
-            longest = [max((x[0] for x in part), default=0) for part in (few, many)]
-            tiles = None
-            if self.num_tokens != self.num_seqs:
-                tiles = to_device([v for x in few + many for v in (*x[1:], 0)], torch.int32, self.cu.device, self.ordered).view(-1, 4)
-            self._rows[group, most, window] = (tiles, len(few), row_tiles, *longest)
-        return self._rows[group, most, window]
+        key = group, heads, window, tuple(blocks)
+        if key not in self._rows:
+            cu, start = torch.tensor(self.cu_host), torch.tensor(self.start_host)
+            new = cu[1:] - cu[:-1]
+            short = (new == 1) | (new * group <= 16)
+            parts, sizes = [], []
+            for rows, pick, most in ((16, short, blocks[0]), (32, ~short, blocks[1])):
+                seqs = pick.nonzero()[:, 0]
+                per = max(1, rows // group)
+                tiles = (new[seqs] + per - 1) // per
+                of = seqs.repeat_interleave(tiles)
+                nth = torch.arange(len(of)) - (tiles.cumsum(0) - tiles).repeat_interleave(tiles)
+                t0 = cu[of] + nth * per
+                t1 = torch.minimum(t0 + per, cu[of + 1])
+                shift = start[of] - cu[of]
+                begin = (t0 + shift - window + 1).clamp(min=0) // step if window > 0 else torch.zeros_like(t0)
+                steps = (t1 - 1 + shift) // step + 1 - begin
+                order = steps.argsort(descending=True, stable=True)
+                of, t0, t1, begin, steps = (x[order] for x in (of, t0, t1, begin, steps))
+                share = int(steps[0]) if len(steps) else 1
+                if 0 < len(steps) * heads < most:  # the smallest parts that the chip takes at once
+                    lo, hi = min(least, share), share
+                    while lo < hi:
+                        mid = (lo + hi) // 2
+                        if int(((steps + mid - 1) // mid).sum()) * heads <= most:
+                            hi = mid
+                        else:
+                            lo = mid + 1
+                    share = lo
+                count = (steps + share - 1) // share
+                each = (steps + count - 1) // count
+                count = (steps + each - 1) // each  # none is empty
+                many = count > 1
+                slots = torch.where(many, count, 0)
+                first = slots.cumsum(0) - slots
+                tile = torch.arange(len(of)).repeat_interleave(count)
+                part = torch.arange(len(tile)) - (count.cumsum(0) - count)[tile]
+                lo = begin[tile] + part * each[tile]
+                hi = torch.minimum(lo + each[tile], (begin + steps)[tile])
+                slot = torch.where(many[tile], first[tile] + part, -1)
+                parts += [torch.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1).flatten(),
+                          torch.stack([t0, t1, first, count], 1)[many].flatten()]
+                sizes += [len(tile), int(many.sum()), int(slots.sum())]
+            self._rows[key] = to_device(torch.cat(parts).tolist(), torch.int32, self.cu.device, self.ordered), sizes
+        return self._rows[key]
 
     @property
     def num_tiles32(self) -> int:

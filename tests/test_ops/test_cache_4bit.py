@@ -399,22 +399,35 @@ def test_refusals():
             paged_attention_4bit(**good | bad)
 
 
-def test_query_tiles():
-    """Every new token is in one tile, and the tiles' rows and keys are what is said."""
-    for counts, starts in (([1, 1], [4, 0]), ([7, 1, 33, 200, 2], [0, 900, 31, 5, 3000]), ([40], [0])):
-        batch = RaggedBatch.build(counts, starts, list(range(len(counts))), "cpu")
-        for group in (1, 3, 8, 16, 20, 70):
-            for window in (0, 10):
-                tiles, few, row_tiles, longest_few, longest_many = batch.query_tiles(group, 4, window)
-                if tiles is None:
-                    assert max(counts) == 1 and few == len(counts)
-                    assert longest_few == (min(max(starts) + 1, window) if window else max(starts) + 1)
-                    continue
-                seen, keys = [], [0, 0]
-                for i, (seq, a, b, _) in enumerate(tiles.tolist()):
-                    assert batch.cu_host[seq] <= a < b <= batch.cu_host[seq + 1]
-                    assert b - a == 1 or (b - a) * group <= (16 if i < few else 16 * row_tiles)
-                    end = batch.start_host[seq] + b - batch.cu_host[seq]
-                    keys[i >= few] = max(keys[i >= few], min(end, window + b - a - 1) if window else end)
-                    seen += range(a, b)
-                assert sorted(seen) == list(range(batch.num_tokens)) and keys == [longest_few, longest_many]
+@pytest.mark.parametrize("counts,starts", [([1, 1], [4, 0]), ([7, 1, 33, 200, 2], [0, 900, 31, 5, 3000]), ([40], [0]), ([1], [40000])])
+@pytest.mark.parametrize("group", [1, 3, 8, 16, 20, 70])
+@pytest.mark.parametrize("window", [0, 10, 1000])
+def test_plan(counts, starts, group, window):
+    """Every key that a new token sees is in exactly one part of the token's one tile; tiles hold their rows; parts are listed with their tiles."""
+    batch = RaggedBatch.build(counts, starts, list(range(len(counts))), "cpu")
+    for blocks in ((1024, 512), (8, 8)):
+        plan, sizes = batch.row_plan(group, 2, window, blocks)
+        at, seen, slots = 0, {}, [[], []]
+        for kind, rows in ((0, 16), (1, 32)):
+            items, joins, used = sizes[3 * kind: 3 * kind + 3]
+            for seq, t0, t1, lo, hi, slot in plan[at: at + 6 * items].view(-1, 6).tolist():
+                assert batch.cu_host[seq] <= t0 < t1 <= batch.cu_host[seq + 1] and lo < hi
+                assert t1 - t0 == 1 or (t1 - t0) * group <= rows
+                seen.setdefault((kind, seq, t0, t1), []).append((lo, hi, slot))
+            at += 6 * items
+            listed = {(t0, t1): (first, count) for t0, t1, first, count in plan[at: at + 4 * joins].view(-1, 4).tolist()}
+            at += 4 * joins
+            mine = {k: v for k, v in seen.items() if k[0] == kind}
+            assert sum(n for _, n in listed.values()) == used and len(listed) == joins
+            taken = sorted(s for v in mine.values() for *_, s in v if s >= 0)
+            assert taken == list(range(used))
+            for (_, seq, t0, t1), v in mine.items():
+                first = batch.start_host[seq] + t0 - batch.cu_host[seq]
+                last = first + t1 - t0 - 1
+                assert v[0][0] == (max(0, first - window + 1) // 32 if window else 0) and v[-1][1] == last // 32 + 1
+                assert all(a[1] == b[0] for a, b in zip(v, v[1:]))
+                if len(v) == 1:
+                    assert v[0][2] == -1 and (t0, t1) not in listed
+                else:
+                    assert listed[t0, t1] == (v[0][2], len(v)) and [s for *_, s in v] == list(range(v[0][2], v[0][2] + len(v)))
+        assert at == plan.numel() and sorted(t for _, _, a, b in seen for t in range(a, b)) == list(range(batch.num_tokens))
