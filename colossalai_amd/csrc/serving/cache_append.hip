@@ -4,10 +4,14 @@
 //   y = R_p (w * x / sqrt(mean(x^2) + eps))
 //
 // A code is that of the exact y: keys that become codes are normed and rotated in float64, so that no rounding ahead of it decides between two
-// numbers; everything else is float32, rounded once. A group with a value that is not finite has the scale byte 255.
+// numbers (it goes on in float32 with an odd last bit where bits were lost, which stands to every border as y does); everything else is
+// float32, rounded once. A group with a value that is not finite has the scale byte 255. Codes are formed two at a time by the conversion
+// instruction, nearest with ties to even.
 //
 // Bound by memory for prompts and by latency for single tokens. A wave takes a token, or with few tokens a share of its heads: D / 16 lanes a head
-// with 8 channels of each half, 64 / lanes heads at a time; the angles stay in registers.
+// with 8 channels of each half, 64 / lanes heads of one kind at a time; the angles stay in registers. 8192 tokens, 32/8 heads of 128 into a 4-bit
+// cache: 43 us, 4.1 TB/s (codes by comparisons in float64 from 180 registers: 109; shares of a token's heads: 44 to 54). 4099 tokens, 28/4
+// heads of 128 into a bfloat16 one: 13.4.
 #include "cache_4bit.h"
 
 #include <c10/core/DeviceGuard.h>
@@ -39,171 +43,153 @@ DEV_INLINE F lanes_sum(F v) {
   return v;
 }
 
+// y of 16 channels, 8 of each half
 template <typename F>
-DEV_INLINE F larger(F a, F b) { return a > b ? a : b; }
-
-// 1 / sqrt(v)
-DEV_INLINE float inverse_root(float v) { return 1.0f / sqrtf(v); }
-DEV_INLINE double inverse_root(double v) { return 1.0 / sqrt(v); }
-
-template <typename T, typename F>
-DEV_INLINE void norm_and_turn(F (&y)[16], const T* w, bool weights, bool narrow, const float* wide, F eps, F inv_d, const float (&c)[8],
-                              const float (&s)[8], int at, int half, int L, bool on, F sum) {
-  if (!on) return;
-  const F r = weights ? inverse_root(sum * inv_d + eps) : F(1);
+DEV_INLINE void norm_and_turn(F (&y)[16], const float (&x)[16], const float (&w)[16], F r, bool weights, const float (&c)[8], const float (&s)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    F a = y[i], b = y[8 + i];
+    F a = x[i], b = x[8 + i];
     if (weights) {
-      a *= r * F(narrow ? ldf(w + at + i) : wide[at + i]);
-      b *= r * F(narrow ? ldf(w + half + at + i) : wide[half + at + i]);
+      a *= r * F(w[i]);
+      b *= r * F(w[8 + i]);
     }
     y[i] = a * F(c[i]) - b * F(s[i]);
     y[8 + i] = b * F(c[i]) + a * F(s[i]);
   }
 }
 
-// Eight codes of y / 2^e, and the group's scale byte from its largest magnitude (4 lanes of 8 channels are a group).
-template <typename F>
-DEV_INLINE unsigned int eight_codes(const F* y, unsigned int& byte) {
-  F most = 0;
-  bool odd = false;
+// y in float32 with an odd last bit where bits were lost: it stands to every number of fewer bits as y does.
+DEV_INLINE float to_odd(double y) {
+  const float f = (float)y;
+  const double back = (double)f;
+  unsigned int bits = __builtin_bit_cast(unsigned int, f);
+  if (fabs(back) > fabs(y)) --bits;
+  if (back != y) bits |= 1u;
+  return fabsf(f) <= 3.4028234663852886e38f ? __builtin_bit_cast(float, bits) : f;
+}
+
+// Eight codes of y / 2^e, nearest, ties to the even mantissa, and the group's scale byte from its largest magnitude (4 lanes of 8 channels are
+// a group).
+DEV_INLINE unsigned int eight_codes(const float* y, unsigned int& byte) {
+  float most = 0;
+  int odd = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const F a = y[i] < 0 ? -y[i] : y[i];
-    odd |= !(a <= F(3.4028234663852886e38));
-    most = larger(most, a);
+    odd |= !(fabsf(y[i]) <= 3.4028234663852886e38f);
+    most = fmaxf(most, fabsf(y[i]));
   }
-  most = larger(most, __shfl_xor(most, 1));
-  most = larger(most, __shfl_xor(most, 2));
-  int odds = odd;
-  odds |= __shfl_xor(odds, 1);
-  odds |= __shfl_xor(odds, 2);
+#pragma unroll
+  for (int off = 1; off < 4; off <<= 1) {
+    most = fmaxf(most, __shfl_xor(most, off));
+    odd |= __shfl_xor(odd, off);
+  }
   // the smallest e with most <= 6 * 2^e: most = f * 2^E, 1 <= f < 2, and 6 = 1.5 * 4
-  const double m = (double)most;
-  const unsigned long long bits = __builtin_bit_cast(unsigned long long, m);
-  int e = (int)(bits >> 52) - 1023 - ((bits & 0xfffffffffffffULL) <= 0x8000000000000ULL ? 2 : 1);
-  e = max(e, -126);
-  byte = odds ? 255u : (unsigned)(e + 127);
-  const F unit = (F)__builtin_bit_cast(double, (unsigned long long)(1023 - e) << 52);   // 2^-e: a power of two from 2^-126 to 2^126
+  const unsigned int bits = __builtin_bit_cast(unsigned int, most);
+  const int e = max((int)(bits >> 23) - 127 - ((bits & 0x7fffffu) <= 0x400000u ? 2 : 1), -126);
+  byte = odd ? 255u : (unsigned)(e + 127);
+  const float unit = __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
   unsigned int word = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const F a = (y[i] < 0 ? -y[i] : y[i]) * unit;
-    // nearest, ties to the even mantissa
-    unsigned int code = (a > F(0.25)) + (a >= F(0.75)) + (a > F(1.25)) + (a >= F(1.75)) + (a > F(2.5)) + (a >= F(3.5)) + (a > F(5));
-    code = odds ? 7u : code;
-    word |= (code | (y[i] < 0 ? 8u : 0u)) << (4 * i);
-  }
-  return word;
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[0], y[1], unit, 0);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], unit, 1);
+  word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], unit, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], unit, 3);
 }
 
 // L: lanes of a head. FOUR: pools of codes, heads of 16 L channels.
 template <typename T, int L, bool FOUR>
-__global__ __launch_bounds__(CA_BLOCK) void append_kernel(T* __restrict__ out, void* __restrict__ kpool, void* __restrict__ vpool,
-                                                          const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Append a) {
+__global__ __launch_bounds__(CA_BLOCK, 4) void append_kernel(T* __restrict__ out, void* __restrict__ kpool, void* __restrict__ vpool,
+                                                             const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, Append a) {
   constexpr int SIDE = WAVE / L, DF = 16 * L;
   const int lane = threadIdx.x & 63, l = lane & (L - 1), side = lane / L, D = FOUR ? DF : a.D, half = D / 2, at = l * 8;
   const bool on = at < half;
-  const long wave = (long)blockIdx.x * CA_WAVES + (threadIdx.x >> 6);
+  const long wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * CA_WAVES + (threadIdx.x >> 6)));
   const long token = wave / a.parts;
   if (token >= a.tokens) return;
-  const int all = a.Hq + 2 * a.G;
   const long row = a.rows[token];
   const bool kept = row >= 0 && row < a.pool_rows;
   const int p = a.positions[token];
   float c[8], s[8];
-  if (on) {
-    if (p >= 0 && p < a.table_rows) {
-      load8(a.table + (long)p * D + at, c);
-      load8(a.table + (long)p * D + half + at, s);
-    } else {   // not in the table
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = __builtin_nanf("");
-    }
+  for (int i = 0; i < 8; ++i) c[i] = s[i] = __builtin_nanf("");   // of a position that the table does not have
+  if (on && p >= 0 && p < a.table_rows) {
+    load8(a.table + (long)p * D + at, c);
+    load8(a.table + (long)p * D + half + at, s);
   }
   const bool weights = a.wq != nullptr;
-  for (int head = (int)(wave % a.parts) * SIDE + side; head < (all + SIDE - 1) / SIDE * SIDE; head += a.parts * SIDE) {
-    const bool is_q = head < a.Hq, is_k = !is_q && head < a.Hq + a.G, here = on && head < all;
-    const int h = is_q ? head : is_k ? head - a.Hq : head - a.Hq - a.G;
-    const T* from = is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride;
-    float x[16];
+  // where the token's rows of codes are, from a head's first tile on
+  const long head_bytes = FOUR ? ((1L << a.page_shift) / TILE) * Tile4<DF>::BYTES : 0;
+  const int off = FOUR ? (int)(row & ((1L << a.page_shift) - 1)) : 0, t = off & (TILE - 1);
+  const long base = FOUR ? (row >> a.page_shift) * a.G * head_bytes + (long)(off / TILE) * Tile4<DF>::BYTES : 0;
+  const int tq = (a.Hq + SIDE - 1) / SIDE, tk = (a.G + SIDE - 1) / SIDE;
+  for (int turn = (int)(wave % a.parts); turn < tq + 2 * tk; turn += a.parts) {
+    const bool is_q = turn < tq, is_k = !is_q && turn < tq + tk;
+    const int h = (turn - (is_q ? 0 : is_k ? tq : tq + tk)) * SIDE + side;
+    const bool here = on && h < (is_q ? a.Hq : a.G);
+    if (!is_q && !kept) continue;
+    const T* from = (is_q ? q + token * a.q_stride : is_k ? k + token * a.k_stride : v + token * a.v_stride) + (long)h * D + at;
+    float x[16], w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.0f;
     if (here) {
-      load8(from + (long)h * D + at, x);
-      load8(from + (long)h * D + half + at, x + 8);
-    }
-    if constexpr (FOUR) {
-      unsigned char* tile = nullptr;
-      int t = 0;
-      if (!is_q && kept) {
-        const long page = row >> a.page_shift;
-        const int off = (int)(row & ((1L << a.page_shift) - 1));
-        t = off & (TILE - 1);
-        tile = (unsigned char*)(is_k ? kpool : vpool) + (page * a.G + h) * (((1L << a.page_shift) / TILE) * Tile4<DF>::BYTES) +
-               off / TILE * Tile4<DF>::BYTES;
-      }
-      unsigned int lo, hi, lo_byte, hi_byte;
-      if (is_k) {
-        double y[16], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          y[i] = here ? x[i] : 0.0f;
-          sum += y[i] * y[i];
-        }
-        if (weights) sum = lanes_sum<L>(sum);
-        norm_and_turn<T, double>(y, (const T*)a.wk, weights, a.narrow_weights, (const float*)a.wk, a.eps, 1.0 / DF, c, s, at, half, L, here, sum);
-        lo = eight_codes(y, lo_byte);
-        hi = eight_codes(y + 8, hi_byte);
-        if (here && kept) {
-          *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::key_codes(t) + at / 2) = lo;
-          *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::key_codes(t) + (half + at) / 2) = hi;
-          if ((l & 3) == 0) {
-            tile[Tile4<DF>::key_scale(t, at / 32)] = (unsigned char)lo_byte;
-            tile[Tile4<DF>::key_scale(t, (half + at) / 32)] = (unsigned char)hi_byte;
-          }
-        }
-        continue;
-      }
-      if (!is_q) {
-        if (!here) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = 0.0f;
-        }
-        lo = eight_codes(x, lo_byte);
-        hi = eight_codes(x + 8, hi_byte);
-        if (here && kept) {
-          if constexpr (DF == 64) {   // a lane's channels are four
-            *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, at)) = (unsigned short)lo;
-            *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, at + 4)) = (unsigned short)(lo >> 16);
-            *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, half + at)) = (unsigned short)hi;
-            *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, half + at + 4)) = (unsigned short)(hi >> 16);
-          } else {
-            *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::value_codes(t, at)) = lo;
-            *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::value_codes(t, half + at)) = hi;
-          }
-          if ((l & 3) == 0) {
-            tile[Tile4<DF>::value_scale(t, at / 32)] = (unsigned char)lo_byte;
-            tile[Tile4<DF>::value_scale(t, (half + at) / 32)] = (unsigned char)hi_byte;
-          }
-        }
-        continue;
-      }
+      load8(from, x);
+      load8(from + half, x + 8);
     }
     if (is_q || is_k) {
-      float sum = 0.0f;
-      if (here) {
+      if (weights && on) {
+        const void* ws = is_q ? a.wq : a.wk;
+        if (a.narrow_weights) {
+          load8((const T*)ws + at, w);
+          load8((const T*)ws + half + at, w + 8);
+        } else {
+          load8((const float*)ws + at, w);
+          load8((const float*)ws + half + at, w + 8);
+        }
+      }
+      if (FOUR && is_k) {
+        double sum = 0, y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += (double)x[i] * x[i];
+        if (weights) sum = lanes_sum<L>(sum);
+        norm_and_turn(y, x, w, weights ? 1.0 / sqrt(sum * (1.0 / DF) + a.eps) : 1.0, weights, c, s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = to_odd(y[i]);
+      } else {
+        float sum = 0.0f, y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += x[i] * x[i];
+        if (weights) sum = lanes_sum<L>(sum);
+        norm_and_turn(y, x, w, weights ? 1.0f / sqrtf(sum * (1.0f / (float)D) + (float)a.eps) : 1.0f, weights, c, s);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = y[i];
       }
-      if (weights) sum = lanes_sum<L>(sum);
-      const void* w = is_q ? a.wq : a.wk;
-      norm_and_turn<T, float>(x, (const T*)w, weights, a.narrow_weights, (const float*)w, (float)a.eps, 1.0f / (float)D, c, s, at, half, L,
-                              here, sum);
     }
-    if (!here || (!is_q && !kept)) continue;
-    T* to = is_q ? out + (token * a.Hq + h) * D : (T*)(is_k ? kpool : vpool) + (row * a.G + h) * D;
-    store8(to + at, x);
-    store8(to + half + at, x + 8);
+    if (!FOUR || is_q) {
+      if (!here) continue;
+      T* to = (is_q ? out + (token * a.Hq + h) * D : (T*)(is_k ? kpool : vpool) + (row * a.G + h) * D) + at;
+      store8(to, x);
+      store8(to + half, x + 8);
+      continue;
+    }
+    unsigned int lo_byte, hi_byte;
+    const unsigned int lo = eight_codes(x, lo_byte), hi = eight_codes(x + 8, hi_byte);
+    if (!here) continue;
+    unsigned char* tile = (unsigned char*)(is_k ? kpool : vpool) + base + h * head_bytes;
+    if (is_k) {
+      *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::key_codes(t) + at / 2) = lo;
+      *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::key_codes(t) + (half + at) / 2) = hi;
+    } else if constexpr (DF == 64) {   // a lane's channels are four
+      *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, at)) = (unsigned short)lo;
+      *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, at + 4)) = (unsigned short)(lo >> 16);
+      *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, half + at)) = (unsigned short)hi;
+      *reinterpret_cast<unsigned short*>(tile + Tile4<DF>::value_codes(t, half + at + 4)) = (unsigned short)(hi >> 16);
+    } else {
+      *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::value_codes(t, at)) = lo;
+      *reinterpret_cast<unsigned int*>(tile + Tile4<DF>::value_codes(t, half + at)) = hi;
+    }
+    if ((l & 3) == 0) {
+      tile[is_k ? Tile4<DF>::key_scale(t, at / 32) : Tile4<DF>::value_scale(t, at / 32)] = (unsigned char)lo_byte;
+      tile[is_k ? Tile4<DF>::key_scale(t, (half + at) / 32) : Tile4<DF>::value_scale(t, (half + at) / 32)] = (unsigned char)hi_byte;
+    }
   }
 }
 
@@ -259,6 +245,8 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
   TORCH_CHECK(q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, who, "q, k and v must be [N, heads, D]");
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in);
+  for (auto* w : {&wq, &wk})
+    if (w->has_value() && reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 != 0) *w = (*w)->clone();
   const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), G = k.size(1);
   TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && k.scalar_type() == q.scalar_type() &&
               v.scalar_type() == q.scalar_type(), who, "keys and values are as many, of one size and of the queries' type");
@@ -312,7 +300,7 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
   auto launch = [&](auto type, auto lanes, auto codes) {
     using T = decltype(type);
     constexpr int L = decltype(lanes)::value;
-    const int64_t turns = (Hq + 2 * G + WAVE / L - 1) / (WAVE / L);
+    const int64_t side = WAVE / L, turns = (Hq + side - 1) / side + 2 * ((G + side - 1) / side);
     a.parts = (int)std::max<int64_t>(1, std::min(turns, 4096 / N));   // 16 waves a CU, while a token's heads give them
     const long blocks = (N * a.parts + CA_WAVES - 1) / CA_WAVES;
     hipLaunchKernelGGL((append_kernel<T, L, decltype(codes)::value>), dim3((unsigned)blocks), dim3(CA_BLOCK), 0, stream(), ptr<T>(out),
