@@ -148,75 +148,70 @@ __global__ __launch_bounds__(NR_BLOCK) void norm_rope_fwd_kernel(T* __restrict__
   }
 }
 
-// dw [blocks, 2, D]: a block's sums.
+// dw [blocks, 2, D]: sums of the blocks of queries (blockIdx.y == 0) and of those of keys, which copy the values' gradients too.
 template <typename T, int L>
 __global__ __launch_bounds__(NR_BLOCK) void norm_rope_bwd_kernel(T* __restrict__ dx, float* __restrict__ dw, const T* __restrict__ dq,
                                                                  const T* __restrict__ dk, const T* __restrict__ dv,
                                                                  const T* __restrict__ x, Heads h) {
   constexpr int SIDE = WAVE / L;
-  __shared__ float lds[NR_WAVES][2][L * 16];
+  __shared__ float lds[NR_WAVES][L * 16];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, l = lane & (L - 1), side = lane / L, half = h.D / 2, at = l * 8;
-  const bool on = at < half;
-  const int all = h.Hq + 2 * h.Hkv;
-  float wq[16], wk[16], gq[16], gk[16];
-  load_weight<T>(wq, h.wq, h.narrow_weights, at, half, on);
-  load_weight<T>(wk, h.wk, h.narrow_weights, at, half, on);
+  const bool on = at < half, keys = blockIdx.y != 0;
+  const int all = h.Hq + 2 * h.Hkv, first = keys ? h.Hq : 0, heads = keys ? h.Hkv : h.Hq;
+  float w[16], g[16];
+  load_weight<T>(w, keys ? h.wk : h.wq, h.narrow_weights, at, half, on);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) gq[i] = gk[i] = 0.0f;
+  for (int i = 0; i < 16; ++i) g[i] = 0.0f;
   const float inv_d = 1.0f / (float)h.D;
   for (long token = (long)blockIdx.x * NR_WAVES + wid; token < h.tokens; token += (long)gridDim.x * NR_WAVES) {
     const long bb = token / h.seq;
     const int ss = (int)(token % h.seq);
-    const T* row = x + bb * h.x_batch + ss * h.x_token;
-    T* out = dx + token * all * h.D;
+    const T* row = x + bb * h.x_batch + ss * h.x_token + (long)first * h.D + at;
+    const T* grad = (keys ? dk : dq) + token * heads * h.D + at;
+    T* out = dx + (token * all + first) * h.D + at;
     float c[8], s[8];
     load_angles(c, s, h, token, ss, at, half, on);
-    // queries, then keys, then values: a kind at a time, so that a lane's sums need no choice
-    auto kind = [&](const T* grad, int first, int heads, const float (&w)[16], float (&g)[16]) {
-      for (int head = side; head < heads; head += SIDE) {
-        Eight<T> lo, hi, glo, ghi;
-        float sum = 0.0f, dot = 0.0f, a[16];
-        if (on) {
-          lo.load(row + (long)(first + head) * h.D + at);
-          hi.load(row + (long)(first + head) * h.D + half + at);
-          const T* from = grad + (token * heads + head) * h.D + at;
-          glo.load(from);
-          ghi.load(from + half);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float p = glo.get(i), r = ghi.get(i), u = lo.get(i), v = hi.get(i);
-            a[i] = p * c[i] + r * s[i];
-            a[8 + i] = r * c[i] - p * s[i];
-            sum += u * u + v * v;
-            dot += a[i] * w[i] * u + a[8 + i] * w[8 + i] * v;
-          }
-        }
-        sum = lanes_sum<L>(sum);
-        dot = lanes_sum<L>(dot);
-        if (!on) continue;
-        const float r = 1.0f / sqrtf(sum * inv_d + h.eps), m = dot * inv_d * r * r;
-        Eight<T> olo, ohi;
+#pragma unroll 1
+    for (int head = side; head < heads; head += SIDE) {
+      Eight<T> lo, hi, glo, ghi;
+      float sum = 0.0f, dot = 0.0f, a[16];
+      if (on) {
+        lo.load(row + (long)head * h.D);
+        hi.load(row + (long)head * h.D + half);
+        glo.load(grad + (long)head * h.D);
+        ghi.load(grad + (long)head * h.D + half);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float u = lo.get(i), v = hi.get(i);
-          olo.set(i, r * (a[i] * w[i] - u * m));
-          ohi.set(i, r * (a[8 + i] * w[8 + i] - v * m));
-          g[i] += a[i] * (u * r);
-          g[8 + i] += a[8 + i] * (v * r);
+          const float p = glo.get(i), r = ghi.get(i), u = lo.get(i), v = hi.get(i);
+          a[i] = p * c[i] + r * s[i];
+          a[8 + i] = r * c[i] - p * s[i];
+          sum += u * u + v * v;
+          dot += a[i] * w[i] * u + a[8 + i] * w[8 + i] * v;
         }
-        olo.store(out + (long)(first + head) * h.D + at);
-        ohi.store(out + (long)(first + head) * h.D + half + at);
       }
-    };
-    kind(dq, 0, h.Hq, wq, gq);
-    kind(dk, h.Hq, h.Hkv, wk, gk);
-    for (int head = side; head < h.Hkv; head += SIDE) {
-      if (!on) break;
+      sum = lanes_sum<L>(sum);
+      dot = lanes_sum<L>(dot);
+      if (!on) continue;
+      const float r = 1.0f / sqrtf(sum * inv_d + h.eps), m = dot * inv_d * r * r;
+      Eight<T> olo, ohi;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = lo.get(i), v = hi.get(i);
+        olo.set(i, r * (a[i] * w[i] - u * m));
+        ohi.set(i, r * (a[8 + i] * w[8 + i] - v * m));
+        g[i] += a[i] * (u * r);
+        g[8 + i] += a[8 + i] * (v * r);
+      }
+      olo.store(out + (long)head * h.D);
+      ohi.store(out + (long)head * h.D + half);
+    }
+    if (!keys || !on) continue;
+    for (int head = side; head < heads; head += SIDE) {
       Eight<T> lo, hi;
-      const T* from = dv + (token * h.Hkv + head) * h.D + at;
+      const T* from = dv + (token * heads + head) * h.D + at;
       lo.load(from);
       hi.load(from + half);
-      T* to = out + (long)(h.Hq + h.Hkv + head) * h.D + at;
+      T* to = out + (long)(heads + head) * h.D;
       lo.store(to);
       hi.store(to + half);
     }
@@ -225,23 +220,15 @@ __global__ __launch_bounds__(NR_BLOCK) void norm_rope_bwd_kernel(T* __restrict__
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
 #pragma unroll
-    for (int off = L; off < WAVE; off <<= 1) {
-      gq[i] += __shfl_xor(gq[i], off);
-      gk[i] += __shfl_xor(gk[i], off);
-    }
-    if (side == 0 && on) {
-      const int ch = at + (i & 7) + (i < 8 ? 0 : half);
-      lds[wid][0][ch] = gq[i];
-      lds[wid][1][ch] = gk[i];
-    }
+    for (int off = L; off < WAVE; off <<= 1) g[i] += __shfl_xor(g[i], off);
+    if (side == 0 && on) lds[wid][at + (i & 7) + (i < 8 ? 0 : half)] = g[i];
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < 2 * h.D; j += NR_BLOCK) {
-    const int which = j >= h.D, ch = j - which * h.D;
+  for (int j = threadIdx.x; j < h.D; j += NR_BLOCK) {
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NR_WAVES; ++w) sum += lds[w][which][ch];
-    dw[(long)blockIdx.x * 2 * h.D + j] = sum;
+    for (int i = 0; i < NR_WAVES; ++i) sum += lds[i][j];
+    dw[((long)blockIdx.x * 2 + keys) * h.D + j] = sum;
   }
 }
 
@@ -379,7 +366,7 @@ std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq_in, at::Tensor dk_in, at::Te
   auto stream = at::hip::getCurrentHIPStream();
   NR_DISPATCH(x.scalar_type(), h.D, {
     if (grid > 0)
-      hipLaunchKernelGGL((norm_rope_bwd_kernel<S, L>), dim3(grid), dim3(NR_BLOCK), 0, stream.stream(), (S*)dx.data_ptr(), part.data_ptr<float>(),
+      hipLaunchKernelGGL((norm_rope_bwd_kernel<S, L>), dim3(grid, 2), dim3(NR_BLOCK), 0, stream.stream(), (S*)dx.data_ptr(), part.data_ptr<float>(),
                          (const S*)dq.data_ptr(), (const S*)dk.data_ptr(), (const S*)dv.data_ptr(), (const S*)x.data_ptr(), h);
     HIP_CHECK_LAST();
     hipLaunchKernelGGL((norm_rope_dw_kernel<S>), dim3((2 * h.D + 31) / 32), dim3(1024), 0, stream.stream(), dwq.data_ptr(), dwk.data_ptr(),
