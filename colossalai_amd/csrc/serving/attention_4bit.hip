@@ -338,33 +338,45 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   }
 }
 
-// Puts the parts of a tile's rows together: eight channels a thread.
+// Puts the parts of a tile's rows together: a wave takes 512 / D rows, eight channels a lane, and eight parts at a time, so that few round trips
+// to memory follow each other.
 template <int D, int RT>
-__global__ __launch_bounds__(256) void attention_4bit_join_kernel(Attend a, long units) {
-  constexpr int R = 16 * RT;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(i % (D / 8)) * 8, r = (int)(i / (D / 8) % R);
-  const long unit = i / (D / 8) / R;
-  if (unit >= units) return;
-  const int g = (int)(unit % a.G), sub = (int)(unit / a.G % a.subs);
-  const int* join = a.joins + unit / a.G / a.subs * 4;
+__global__ __launch_bounds__(64) void attention_4bit_join_kernel(Attend a) {
+  constexpr int R = 16 * RT, LANES = D / 8, AT_ONCE = 8;
+  const int c = (int)threadIdx.x % LANES * 8, r = blockIdx.y * (64 / LANES) + (int)threadIdx.x / LANES;
+  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
+  const int* join = a.joins + (long)(blockIdx.x / a.G / a.subs) * 4;
   const int t0 = join[0], t1 = join[1], count = join[3];
   const int per_token = min(a.group, R), tok = t0 + r / per_token, in = sub * R + r % per_token;
   if (tok >= t1 || in >= a.group) return;
   const float* part = a.parts + (((long)join[2] * a.subs + sub) * a.G + g) * (R * (D + 2L));
   const long next = (long)a.subs * a.G * (R * (D + 2L));
-  float top = -INFINITY, sum = 0.0f, o[8] = {};
-  for (int s = 0; s < count; ++s) top = fmaxf(top, part[s * next + (long)R * D + r * 2]);
-#pragma unroll 4
-  for (int s = 0; s < count; ++s) {
-    const float* p = part + s * next;
-    const float m = p[(long)R * D + r * 2], l = p[(long)R * D + r * 2 + 1];
-    const float w = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);   // without a reference all is 0, or NaN, which stays
-    sum += w * l;
-    float x[8];
-    load8(p + r * D + c, x);
+  float m = -INFINITY, sum = 0.0f, o[8] = {};
+  for (int first = 0; first < count; first += AT_ONCE) {
+    float2v state[AT_ONCE];
+    float x[AT_ONCE][8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] += w * x[e];
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const float* p = part + min(first + i, count - 1) * next;
+      state[i] = *reinterpret_cast<const float2v*>(p + (long)R * D + r * 2);
+      load8(p + r * D + c, x[i]);
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, state[i][0]);
+    const float fall = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);   // without a reference all is 0, or NaN, which stays
+    sum *= fall;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= fall;
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      if (first + i >= count) break;
+      const float w = state[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(state[i][0] - top);
+      sum += w * state[i][1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += w * x[i][e];
+    }
+    m = top;
   }
   const float inv = 1.0f / sum;
 #pragma unroll
@@ -384,8 +396,7 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
   hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(items * heads)), dim3(64 * WAVES4), 0, stream(), a);
   HIP_CHECK_LAST();
   if (joins > 0) {
-    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)((joins * heads * 16 * RT * (D / 8) + 255) / 256)), dim3(256), 0, stream(),
-                       a, joins * heads);
+    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)(joins * heads), 16 * RT * D / 512), dim3(64), 0, stream(), a);
     HIP_CHECK_LAST();
   }
 }
@@ -398,21 +409,21 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
 at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions,
                                 at::Tensor plan, std::vector<int64_t> sizes, double scale, int64_t window, int64_t page_size) {
   const char* who = "paged_attention_4bit: ";
-  TORCH_CHECK(q_in.is_cuda() && q_in.dim() == 3 && is_bf16(q_in), who, "q must be bfloat16 [N, H, D]");
+  TORCH_CHECK_VALUE(q_in.is_cuda() && q_in.dim() == 3 && is_bf16(q_in), who, "q must be bfloat16 [N, H, D]");
   const c10::DeviceGuard guard(q_in.device());
   const int64_t N = q_in.size(0), H = q_in.size(1), D = q_in.size(2);
-  TORCH_CHECK(D == 64 || D == 128 || D == 256, who, "heads of 64, 128 or 256 channels, got ", D);
-  TORCH_CHECK(page_size_of(kpool, D) == page_size && page_size_of(vpool, D) == page_size && kpool.sizes() == vpool.sizes() && kpool.size(0) > 0, who,
+  TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, who, "heads of 64, 128 or 256 channels, got ", D);
+  TORCH_CHECK_VALUE(page_size_of(kpool, D) == page_size && page_size_of(vpool, D) == page_size && kpool.sizes() == vpool.sizes() && kpool.size(0) > 0, who,
               "pools must be contiguous uint8 [pages, heads, page size * 17 * D / 32] of the batch's page size ", page_size);
   const int64_t G = kpool.size(1);
-  TORCH_CHECK(G > 0 && H % G == 0, who, H, " query heads cannot share ", G, " key heads");
+  TORCH_CHECK_VALUE(G > 0 && H % G == 0, who, H, " query heads cannot share ", G, " key heads");
   check_i32(block_tables, "block_tables");
   check_i32(plan, "plan");
   check_i32(positions, "positions");
-  TORCH_CHECK(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 6 &&
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 6 &&
               plan.numel() == 6 * (sizes[0] + sizes[3]) + 4 * (sizes[1] + sizes[4]), who, "batch of other tokens");
   for (const at::Tensor& t : {kpool, vpool, block_tables, positions, plan})
-    TORCH_CHECK(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
+    TORCH_CHECK_VALUE(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
   const bool fits = q_in.stride(2) == 1 && q_in.stride(1) == D && q_in.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
   const at::Tensor q = fits ? q_in : q_in.clone(at::MemoryFormat::Contiguous), out = at::empty({N, H, D}, q.options());
   if (N == 0) return out;

@@ -241,41 +241,44 @@ int log2_of(int64_t v) {
 at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at::Tensor kpool, at::Tensor vpool, at::Tensor rows,
                            at::Tensor positions, at::Tensor table, c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, double eps) {
   const char* who = "paged_kv_append: ";
-  check_act(q_in, "q");
-  TORCH_CHECK(q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, who, "q, k and v must be [N, heads, D]");
+  TORCH_CHECK_VALUE(q_in.is_cuda() && q_in.dim() == 3 && k_in.dim() == 3 && v_in.dim() == 3, who, "q, k and v must be [N, heads, D] on a GPU");
+  TORCH_CHECK_VALUE((is_bf16(q_in) || is_f32(q_in)) && k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type(), who,
+                    "q, k and v must be bfloat16 or float32 and of one type");
+  TORCH_CHECK_VALUE(k_in.sizes() == v_in.sizes() && k_in.size(0) == q_in.size(0) && k_in.size(2) == q_in.size(2), who,
+                    "keys and values must be as many as the queries, of one size");
+  for (const at::Tensor& t : {k_in, v_in, kpool, vpool, rows, positions, table, wq.value_or(q_in), wk.value_or(q_in)})
+    TORCH_CHECK_VALUE(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in);
-  for (auto* w : {&wq, &wk})
-    if (w->has_value() && reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 != 0) *w = (*w)->clone();
   const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), G = k.size(1);
-  TORCH_CHECK(k.sizes() == v.sizes() && k.size(0) == N && k.size(2) == D && k.scalar_type() == q.scalar_type() &&
-              v.scalar_type() == q.scalar_type(), who, "keys and values are as many, of one size and of the queries' type");
-  for (const at::Tensor& t : {k, v, kpool, vpool, rows, positions, table, wq.value_or(q), wk.value_or(q)})
-    TORCH_CHECK(t.device() == q.device(), who, "tensors on ", q.device(), " and ", t.device());
-  check_i32(rows, "rows");
-  check_i32(positions, "positions");
-  TORCH_CHECK(rows.numel() == N && positions.numel() == N, who, "rows and positions must be one a token");
-  TORCH_CHECK(table.dim() == 2 && is_f32(table) && table.is_contiguous() && table.size(1) == D, who, "table must be float32 [positions, D]");
-  TORCH_CHECK(wq.has_value() == wk.has_value(), who, "both weights or none");
+  TORCH_CHECK_VALUE(rows.scalar_type() == at::kInt && positions.scalar_type() == at::kInt && rows.numel() == N && positions.numel() == N, who,
+                    "rows and positions must be int32, one a token");
+  rows = rows.contiguous();
+  positions = positions.contiguous();
+  TORCH_CHECK_VALUE(table.dim() == 2 && is_f32(table) && table.size(1) == D, who, "table must be float32 [positions, D]");
+  table = table.contiguous();
+  if (reinterpret_cast<uintptr_t>(table.data_ptr()) % 16 != 0) table = table.clone();
+  TORCH_CHECK_VALUE(wq.has_value() == wk.has_value(), who, "both weights or none");
   if (wq.has_value()) {
-    TORCH_CHECK(wq->numel() == D && wk->numel() == D && wq->is_contiguous() && wk->is_contiguous() && wq->scalar_type() == wk->scalar_type() &&
-                (is_f32(*wq) || wq->scalar_type() == q.scalar_type()), who, "weights must be [D], of the queries' type or float32");
+    TORCH_CHECK_VALUE(wq->dim() == 1 && wk->dim() == 1 && wq->numel() == D && wk->numel() == D && wq->scalar_type() == wk->scalar_type() && (is_f32(*wq) || wq->scalar_type() == q.scalar_type()), who, "weights must be [D], of the queries' type or float32");
   }
+  for (auto* w : {&wq, &wk})   // 16-byte loads
+    if (w->has_value()) *w = reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 == 0 ? (*w)->contiguous() : (*w)->clone(at::MemoryFormat::Contiguous);
   const bool four = kpool.scalar_type() == at::kByte;
   Append a;
   if (four) {
-    TORCH_CHECK(D == 64 || D == 128 || D == 256, who, "4-bit pools take heads of 64, 128 or 256 channels, got ", D);
+    TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, who, "4-bit pools take heads of 64, 128 or 256 channels, got ", D);
     const int64_t ps = page_size_of(kpool, D);
-    TORCH_CHECK(ps > 0 && kpool.size(1) == G && vpool.sizes() == kpool.sizes() && page_size_of(vpool, D) == ps, who,
+    TORCH_CHECK_VALUE(ps > 0 && kpool.size(1) == G && vpool.sizes() == kpool.sizes() && page_size_of(vpool, D) == ps, who,
                 "4-bit pools must be contiguous uint8 [pages, ", G, ", page size * 17 * ", D, " / 32], page sizes powers of two from 16 on");
     a.page_shift = log2_of(ps);
     a.pool_rows = kpool.size(0) * ps;
   } else {
-    TORCH_CHECK(kpool.dim() == 4 && kpool.is_contiguous() && vpool.is_contiguous() && kpool.sizes() == vpool.sizes() &&
+    TORCH_CHECK_VALUE(kpool.dim() == 4 && kpool.is_contiguous() && vpool.is_contiguous() && kpool.sizes() == vpool.sizes() &&
                 kpool.size(2) == G && kpool.size(3) == D && kpool.scalar_type() == q.scalar_type() && vpool.scalar_type() == q.scalar_type(),
                 who, "pools must be contiguous [pages, page size, ", G, ", ", D, "] of the keys' type, or uint8");
-    TORCH_CHECK(D % 16 == 0 && D <= 512, who, "head sizes are multiples of 16 up to 512, got ", D);
-    TORCH_CHECK(reinterpret_cast<uintptr_t>(kpool.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(vpool.data_ptr()) % 16 == 0, who,
+    TORCH_CHECK_VALUE(D % 16 == 0 && D <= 512, who, "head sizes are multiples of 16 up to 512, got ", D);
+    TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(kpool.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(vpool.data_ptr()) % 16 == 0, who,
                 "pools must start at 16-byte addresses");
     a.page_shift = 0;
     a.pool_rows = kpool.size(0) * kpool.size(1);
@@ -324,13 +327,14 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
 }
 
 std::vector<at::Tensor> kv4_read(at::Tensor kpool, at::Tensor vpool, at::Tensor rows, int64_t D) {
-  TORCH_CHECK(D == 64 || D == 128 || D == 256, "kv4_read: 4-bit pools hold heads of 64, 128 or 256 channels, got ", D);
+  TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, "kv4_read: 4-bit pools hold heads of 64, 128 or 256 channels, got ", D);
   const int64_t ps = page_size_of(kpool, D);
-  TORCH_CHECK(kpool.is_cuda() && ps > 0 && vpool.sizes() == kpool.sizes() && page_size_of(vpool, D) == ps,
+  TORCH_CHECK_VALUE(kpool.is_cuda() && ps > 0 && vpool.sizes() == kpool.sizes() && page_size_of(vpool, D) == ps,
               "kv4_read: pools must be contiguous uint8 [pages, heads, page size * 17 * D / 32]");
   const c10::DeviceGuard guard(kpool.device());
-  check_i32(rows, "rows");
-  TORCH_CHECK(vpool.device() == kpool.device() && rows.device() == kpool.device(), "kv4_read: tensors on several devices");
+  TORCH_CHECK_VALUE(rows.scalar_type() == at::kInt && rows.dim() == 1, "kv4_read: rows must be int32 [N]");
+  rows = rows.contiguous();
+  TORCH_CHECK_VALUE(vpool.device() == kpool.device() && rows.device() == kpool.device(), "kv4_read: tensors on several devices");
   const int64_t N = rows.numel(), G = kpool.size(1);
   const auto k = at::empty({N, G, D}, kpool.options().dtype(at::kBFloat16)), v = at::empty_like(k);
   if (N == 0) return {k, v};

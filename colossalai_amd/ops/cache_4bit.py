@@ -28,6 +28,7 @@ __all__ = ["kv4_pool", "kv4_read", "kv4_unpack", "paged_kv_append", "paged_kv_ap
 
 HEAD_DIMS = (64, 128, 256)
 _NUMBERS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+_BLOCKS = {64: (1024, 512), 128: (768, 512), 256: (512, 256)}
 _BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)
 
 
@@ -99,13 +100,13 @@ def kv4_unpack(pool: torch.Tensor, head_dim: int, values: bool) -> torch.Tensor:
 def kv4_read(kpool: torch.Tensor, vpool: torch.Tensor, rows: torch.Tensor, head_dim: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The numbers that rows (int32 [N]) of a layer's pools hold: keys and values, bfloat16 [N, heads, head_dim] (which has every one of them
     but products below its smallest). NaN for a row that the pools do not have."""
+    if use_hip(kpool):
+        return tuple(serving_kernels().kv4_read(kpool, vpool, rows, head_dim))
     ps = _page_size(kpool, head_dim)
     if vpool.shape != kpool.shape or vpool.dtype != torch.uint8:
         raise ValueError(f"both pools have one shape, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
     if rows.dtype != torch.int32 or rows.dim() != 1:
         raise ValueError(f"rows must be int32 [N], got {rows.dtype} {tuple(rows.shape)}")
-    if use_hip(kpool):
-        return tuple(serving_kernels().kv4_read(kpool, vpool, rows.contiguous(), head_dim))
     here = (rows >= 0) & (rows < kpool.shape[0] * ps)
     at = torch.where(here, rows, 0).long()
     return tuple(kv4_unpack(p, head_dim, v).flatten(0, 1)[at].masked_fill(~here[:, None, None], float("nan")).bfloat16()
@@ -136,17 +137,7 @@ def paged_kv_append_ref(q, k, v, kpool, vpool, rows, positions, table, q_weight=
     return out
 
 
-def paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, rows: torch.Tensor,
-                    positions: torch.Tensor, table: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
-                    k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
-    """New tokens on their way into a paged cache, in one launch: q [N, H, D] and k [N, G, D] are divided by their heads' root mean square and
-    multiplied by ``q_weight`` / ``k_weight`` [D] (if both are given) and rotated by ``positions`` (pairs ``(i, i + D / 2)``, ``table`` of
-    ``build_rope_table``); keys and values [N, G, D] go to pool rows ``rows``. Returns the queries, contiguous in q's type.
-
-    Types are bfloat16 or float32 (token strides of q, k and v are free), weights of the same type or float32, positions and rows int32 [N].
-    Pools are [pages, page size, G, D] of the keys' type (D a multiple of 16 up to 512), or 4-bit ones of ``kv4_pool``. A row that the pools do
-    not have, as -1 for a padding token, is not written; no two tokens may have the same one. A position that the table does not have gives
-    NaN."""
+def _check_append(q, k, v, kpool, vpool, rows, positions, table, q_weight, k_weight):
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
         raise ValueError(f"q [N, H, D] and k, v [N, G, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in (torch.bfloat16, torch.float32) or not q.dtype == k.dtype == v.dtype:
@@ -175,13 +166,23 @@ def paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kpool: to
     if q_weight is not None and (q_weight.shape != (D,) or k_weight.shape != (D,) or q_weight.dtype != k_weight.dtype
                                  or q_weight.dtype not in (q.dtype, torch.float32)):
         raise ValueError(f"weights must be [{D}], of the queries' type or float32")
-    rows, positions = rows.reshape(-1), positions.reshape(-1)
-    if not use_hip(q):
-        return paged_kv_append_ref(q, k, v, kpool, vpool, rows, positions, table, q_weight, k_weight, eps)
-    if q_weight is not None:
-        q_weight, k_weight = q_weight.detach().contiguous(), k_weight.detach().contiguous()
-    return serving_kernels().paged_kv_append(q, k, v, kpool, vpool, rows.contiguous(), positions.contiguous(), table.contiguous(), q_weight, k_weight,
-                                             float(eps))
+
+
+def paged_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, rows: torch.Tensor,
+                    positions: torch.Tensor, table: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                    k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
+    """New tokens on their way into a paged cache, in one launch: q [N, H, D] and k [N, G, D] are divided by their heads' root mean square and
+    multiplied by ``q_weight`` / ``k_weight`` [D] (if both are given) and rotated by ``positions`` (pairs ``(i, i + D / 2)``, ``table`` of
+    ``build_rope_table``); keys and values [N, G, D] go to pool rows ``rows``. Returns the queries, contiguous in q's type.
+
+    Types are bfloat16 or float32 (token strides of q, k and v are free), weights of the same type or float32, positions and rows int32 [N].
+    Pools are [pages, page size, G, D] of the keys' type (D a multiple of 16 up to 512), or 4-bit ones of ``kv4_pool``. A row that the pools do
+    not have, as -1 for a padding token, is not written; no two tokens may have the same one. A position that the table does not have gives
+    NaN."""
+    if use_hip(q):  # the arguments are looked over there: it takes the host 1 us for 6
+        return serving_kernels().paged_kv_append(q, k, v, kpool, vpool, rows, positions, table, q_weight, k_weight, eps)
+    _check_append(q, k, v, kpool, vpool, rows, positions, table, q_weight, k_weight)
+    return paged_kv_append_ref(q, k, v, kpool, vpool, rows.reshape(-1), positions.reshape(-1), table, q_weight, k_weight, eps)
 
 
 def paged_attention_4bit_ref(q, kpool, vpool, batch: RaggedBatch, scale: float, window: int = 0):
@@ -211,22 +212,18 @@ def paged_attention_4bit(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tens
     rounded to bfloat16 for its product. A page number that the pools do not have gives NaN to the tokens that see it."""
     if q.dim() != 3 or q.shape[0] != batch.num_tokens:
         raise ValueError(f"q must be [{batch.num_tokens}, H, D], got {tuple(q.shape)}")
-    ps = _page_size(kpool, q.shape[2])
-    if vpool.shape != kpool.shape or vpool.dtype != torch.uint8:
-        raise ValueError(f"both pools have one shape, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
-    if batch.block_tables is None or batch.page_size != ps:
-        raise ValueError(f"the batch has pages of {batch.page_size} tokens, the pools of {ps}")
-    G = kpool.shape[1]
-    if G == 0 or q.shape[1] % G:
-        raise ValueError(f"{q.shape[1]} query heads cannot share {G} key heads")
-    if window < 0:
-        raise ValueError(f"window must be 0 or more, got {window}")
-    if not use_hip(q):
-        return paged_attention_4bit_ref(q, kpool, vpool, batch, scale, window)
-    if q.dtype != torch.bfloat16:
-        raise ValueError(f"on a GPU the queries are bfloat16, got {q.dtype}")
-    # what a chip of 256 CUs holds at once, by the kernel's registers
-    blocks = {64: (1024, 512), 128: (768, 512), 256: (512, 256)}[q.shape[2]]
-    subs = -(-(q.shape[1] // G) // 16)
-    plan, sizes = batch.row_plan(q.shape[1] // G, G * subs, window, blocks)
-    return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.positions, plan, sizes, float(scale), int(window), ps)
+    _, H, D = q.shape
+    G = kpool.shape[1] if kpool.dim() == 3 else 0
+    if D not in HEAD_DIMS or G == 0 or H % G:
+        raise ValueError(f"heads of 64, 128 or 256 channels, the pools' heads shared by as many query heads each, got {H} heads of {D} and pools "
+                         f"{tuple(kpool.shape)}")
+    if batch.block_tables is None or window < 0:
+        raise ValueError("a batch with page tables, and a window of 0 or more")
+    if use_hip(q):
+        # the blocks that 256 CUs hold at once, by the kernel's registers
+        plan, sizes = batch.row_plan(H // G, G * -(-H // G // 16), window, _BLOCKS[D])
+        return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.positions, plan, sizes, scale, window, batch.page_size)
+    ps = _page_size(kpool, D)
+    if vpool.shape != kpool.shape or vpool.dtype != torch.uint8 or batch.page_size != ps:
+        raise ValueError(f"both pools have one shape and the batch's pages of {batch.page_size} tokens, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
+    return paged_attention_4bit_ref(q, kpool, vpool, batch, scale, window)

@@ -369,34 +369,40 @@ def test_together_on_another_stream_and_in_a_captured_graph():
         assert torch.equal(held[turn % 2], want)
 
 
-def test_refusals():
+@pytest.mark.parametrize("device", EACH)
+def test_refusals(device):
     D, N = 64, 3
-    table, q, k = build_rope_table(16, D), torch.zeros(N, 4, D), torch.zeros(N, 2, D)
-    pool, plain, rows = kv4_pool(4, 16, 2, D), torch.zeros(4, 16, 2, D), torch.arange(N).int()
+    table, q, k = build_rope_table(16, D).to(device), torch.zeros(N, 4, D, device=device).bfloat16(), torch.zeros(N, 2, D, device=device).bfloat16()
+    pool, plain, rows = kv4_pool(4, 16, 2, D, device), torch.zeros(4, 16, 2, D, device=device).bfloat16(), torch.arange(N, device=device).int()
     good = dict(q=q, k=k, v=k, kpool=pool, vpool=pool, rows=rows, positions=rows, table=table)
-    w = torch.ones(D)
-    for bad in (dict(q=q[0]), dict(q=q[:2]), dict(k=k[..., :32], v=k[..., :32]), dict(v=k[:, :1]), dict(q=q.half()), dict(k=k.bfloat16(), v=k.bfloat16()),
-                dict(vpool=kv4_pool(5, 16, 2, D)), dict(kpool=pool[..., :-1], vpool=pool[..., :-1]), dict(kpool=plain[:, :, :1], vpool=plain[:, :, :1]),
-                dict(kpool=kv4_pool(4, 16, 1, D), vpool=kv4_pool(4, 16, 1, D)), dict(kpool=plain.bfloat16(), vpool=plain.bfloat16()), dict(rows=rows.long()),
-                dict(rows=rows[:2]), dict(positions=rows.float()), dict(table=table.half()), dict(table=table[:, :32]), dict(q_weight=w),
-                dict(q_weight=w, k_weight=w[:32]), dict(q_weight=w.half(), k_weight=w.half())):
+    w = torch.ones(D, device=device)
+    one = kv4_pool(4, 16, 1, D, device)
+    for bad in (dict(q=q[0]), dict(q=q[:2]), dict(k=k[..., :32], v=k[..., :32]), dict(v=k[:, :1]), dict(q=q.half()), dict(k=k.float(), v=k.float()),
+                dict(q=q.half(), k=k.half(), v=k.half()), dict(vpool=kv4_pool(5, 16, 2, D, device)), dict(kpool=pool[..., :-1], vpool=pool[..., :-1]),
+                dict(kpool=plain[:, :, :1], vpool=plain[:, :, :1]), dict(kpool=one, vpool=one), dict(kpool=plain.float(), vpool=plain.float()),
+                dict(kpool=plain), dict(rows=rows.long()), dict(rows=rows[:2]), dict(positions=rows.float()), dict(table=table.half()),
+                dict(table=table[:, :32]), dict(q_weight=w), dict(q_weight=w, k_weight=w[:32]), dict(q_weight=w.half(), k_weight=w.half())):
         with pytest.raises(ValueError):
             paged_kv_append(**good | bad)
     for shape in ((4, 8, 2, 64), (4, 24, 2, 64), (4, 16, 2, 96)):
         with pytest.raises(ValueError):
             kv4_pool(*shape)
-    with pytest.raises(ValueError):
-        kv4_read(pool, pool, rows.long(), D)
-    with pytest.raises(ValueError):
-        kv4_read(pool, pool[:2], rows, D)
-    with pytest.raises(ValueError):
-        kv4_read(pool, pool, rows, 128)
-    batch = RaggedBatch.build([3], [0], [0], "cpu", [[1]], 16)
+    for bad in ((pool, pool, rows.long(), D), (pool, pool[:2], rows, D), (pool, pool, rows, 128), (pool, pool, rows, 96), (pool.int(), pool.int(), rows, D)):
+        with pytest.raises(ValueError):
+            kv4_read(*bad)
+    batch = RaggedBatch.build([3], [0], [0], device, [[1]], 16)
     good = dict(q=q, kpool=pool, vpool=pool, batch=batch, scale=0.1, window=0)
-    for bad in (dict(q=q[:2]), dict(q=torch.zeros(N, 3, D)), dict(q=torch.zeros(N, 4, 96)), dict(vpool=pool[:3]), dict(window=-1), dict(kpool=pool.int(), vpool=pool.int()),
-                dict(batch=RaggedBatch.build([3], [0], [0], "cpu", [[1]], 32)), dict(batch=RaggedBatch.build([3], [0], [0], "cpu"))):
+    wide = RaggedBatch.build([3], [0], [0], device, [[1]], 32)
+    for bad in (dict(q=q[:2]), dict(q=q[:, :3]), dict(q=torch.zeros(N, 4, 96, device=device)), dict(vpool=pool[:3]), dict(window=-1),
+                dict(kpool=pool.int(), vpool=pool.int()), dict(kpool=pool[0], vpool=pool[0]), dict(batch=wide),
+                dict(batch=RaggedBatch.build([3], [0], [0], device))):
         with pytest.raises(ValueError):
             paged_attention_4bit(**good | bad)
+    if device == "cuda":
+        with pytest.raises(ValueError):
+            paged_attention_4bit(**good | dict(q=q.float()))
+        with pytest.raises(ValueError):
+            paged_kv_append(q, k, k, pool, pool, rows, rows, table.cpu())
 
 
 @pytest.mark.parametrize("counts,starts", [([1, 1], [4, 0]), ([7, 1, 33, 200, 2], [0, 900, 31, 5, 3000]), ([40], [0]), ([1], [40000])])
