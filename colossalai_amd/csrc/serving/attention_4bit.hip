@@ -114,11 +114,15 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   const int* table = a.tables + (long)seq * a.width;
   const float scale = a.scale * LOG2E4;
 
-  auto load = [&](Raw<D>& w, int step) {
+  // a tile behind the end is its last one again: hidden by its places
+  auto look = [&](int (&pages)[2], int step) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pages[h] = table[min(step * STEP + h * TILE, p1) >> a.page_shift];
+  };
+  auto load = [&](Raw<D>& w, int step, const int (&pages)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = min(step * STEP + h * TILE, p1);   // a tile behind the end is its last one again: hidden by its places
-      const int page = table[at >> a.page_shift];
+      const int at = min(step * STEP + h * TILE, p1), page = pages[h];
       w.bad[h] = (unsigned)page >= (unsigned long)a.pages;
       const long base = (long)(w.bad[h] ? 0 : page) * a.page_stride + (long)g * a.head_bytes +
                         (long)((at & ((1 << a.page_shift) - 1)) / TILE) * Tile4<D>::BYTES;
@@ -251,15 +255,27 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
     });
   };
 
-  // the next step's codes are on their way while a step is worked on
+  // the next step's codes are on their way while a step is worked on, and the page numbers of the one after it
   int step = from + wid;
   if (step < to) {
-    Raw<D> now, next;
-    load(now, step);
-    for (; step < to; step += WAVES4) {
-      if (step + WAVES4 < to) load(next, step + WAVES4);
-      compute(now, step);
-      now = next;
+    Raw<D> even, odd;
+    int pages[2];
+    look(pages, step);
+    load(even, step, pages);
+    look(pages, step + WAVES4);
+    while (true) {
+      if (step + WAVES4 < to) {
+        load(odd, step + WAVES4, pages);
+        look(pages, step + 2 * WAVES4);
+      }
+      compute(even, step);
+      if ((step += WAVES4) >= to) break;
+      if (step + WAVES4 < to) {
+        load(even, step + WAVES4, pages);
+        look(pages, step + 2 * WAVES4);
+      }
+      compute(odd, step);
+      if ((step += WAVES4) >= to) break;
     }
   }
 
@@ -338,21 +354,27 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   }
 }
 
-// Puts the parts of a tile's rows together: a wave takes 512 / D rows, eight channels a lane, and eight parts at a time, so that few round trips
-// to memory follow each other.
+// Puts the parts of a tile's rows together: a block takes 512 / D rows, eight channels a lane; its waves take eight parts each at a time, so that
+// few round trips to memory follow each other, and meet in LDS.
+constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
+
 template <int D, int RT>
-__global__ __launch_bounds__(64) void attention_4bit_join_kernel(Attend a) {
-  constexpr int R = 16 * RT, LANES = D / 8, AT_ONCE = 8;
-  const int c = (int)threadIdx.x % LANES * 8, r = blockIdx.y * (64 / LANES) + (int)threadIdx.x / LANES;
+__global__ __launch_bounds__(64 * JOIN_WAVES) void attention_4bit_join_kernel(Attend a) {
+  constexpr int R = 16 * RT, LANES = D / 8;
+  __shared__ float lds[JOIN_WAVES][10][64];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane % LANES * 8, r = blockIdx.y * (64 / LANES) + lane / LANES;
   const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
   const int* join = a.joins + (long)(blockIdx.x / a.G / a.subs) * 4;
   const int t0 = join[0], t1 = join[1], count = join[3];
   const int per_token = min(a.group, R), tok = t0 + r / per_token, in = sub * R + r % per_token;
-  if (tok >= t1 || in >= a.group) return;
+  if (blockIdx.y * (64 / LANES) >= (t1 - t0) * per_token) return;   // the whole block
+  const bool real = tok < t1 && in < a.group;
   const float* part = a.parts + (((long)join[2] * a.subs + sub) * a.G + g) * (R * (D + 2L));
   const long next = (long)a.subs * a.G * (R * (D + 2L));
   float m = -INFINITY, sum = 0.0f, o[8] = {};
-  for (int first = 0; first < count; first += AT_ONCE) {
+  // the sums fall to a new reference; without an old one all is 0, or NaN, which stays
+  auto fall = [](float from, float to) { return from == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(from - to); };
+  for (int first = wid * AT_ONCE; real && first < count; first += JOIN_WAVES * AT_ONCE) {
     float2v state[AT_ONCE];
     float x[AT_ONCE][8];
 #pragma unroll
@@ -364,20 +386,42 @@ __global__ __launch_bounds__(64) void attention_4bit_join_kernel(Attend a) {
     float top = m;
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) top = fmaxf(top, state[i][0]);
-    const float fall = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top);   // without a reference all is 0, or NaN, which stays
-    sum *= fall;
+    const float w = fall(m, top);
+    sum *= w;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] *= fall;
+    for (int e = 0; e < 8; ++e) o[e] *= w;
 #pragma unroll
     for (int i = 0; i < AT_ONCE; ++i) {
       if (first + i >= count) break;
-      const float w = state[i][0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(state[i][0] - top);
-      sum += w * state[i][1];
+      const float u = fall(state[i][0], top);
+      sum += u * state[i][1];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] += w * x[i][e];
+      for (int e = 0; e < 8; ++e) o[e] += u * x[i][e];
     }
     m = top;
   }
+  if (count > AT_ONCE) {   // other waves had parts
+    lds[wid][8][lane] = m;
+    lds[wid][9][lane] = sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) lds[wid][e][lane] = o[e];
+    __syncthreads();
+    if (wid != 0) return;
+    float top = m;
+#pragma unroll
+    for (int w = 1; w < JOIN_WAVES; ++w) top = fmaxf(top, lds[w][8][lane]);
+    sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WAVES; ++w) {
+      const float u = fall(lds[w][8][lane], top);
+      sum += u * lds[w][9][lane];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] += u * lds[w][e][lane];
+    }
+  }
+  if (wid != 0 || !real) return;
   const float inv = 1.0f / sum;
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] *= inv;
@@ -396,7 +440,7 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
   hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(items * heads)), dim3(64 * WAVES4), 0, stream(), a);
   HIP_CHECK_LAST();
   if (joins > 0) {
-    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)(joins * heads), 16 * RT * D / 512), dim3(64), 0, stream(), a);
+    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)(joins * heads), 16 * RT * D / 512), dim3(64 * JOIN_WAVES), 0, stream(), a);
     HIP_CHECK_LAST();
   }
 }
