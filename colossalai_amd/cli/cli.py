@@ -92,7 +92,8 @@ def check(installation):
 @click.option("--top-p", type=float, default=1.0)
 @click.option("--max-batch-size", type=int, default=8)
 @click.option("--max-step-tokens", type=int, default=2048, help="token budget of one engine step (chunked prefill)")
-def generate(model_dir, prompt_ids, max_new_tokens, dtype, temperature, top_k, top_p, max_batch_size, max_step_tokens):
+@click.option("--kv-bits", type=click.Choice(["16", "4"]), default="16", help="keys and values of Llama-family models in the model's type, or in 4 bits")
+def generate(model_dir, prompt_ids, max_new_tokens, dtype, temperature, top_k, top_p, max_batch_size, max_step_tokens, kv_bits):
     """Generate from token ids with any registered model (class chosen by config.json)."""
     import json
 
@@ -107,7 +108,8 @@ def generate(model_dir, prompt_ids, max_new_tokens, dtype, temperature, top_k, t
     prompts = [[int(t) for t in part.split(",") if t.strip()] for part in prompt_ids.split(";") if part.strip()]
     longest = max(len(p) for p in prompts)
     engine = ContinuousBatchEngine(
-        model, InferenceConfig(max_batch_size=max_batch_size, max_input_len=longest, max_output_len=max_new_tokens, dtype=td),
+        model, InferenceConfig(max_batch_size=max_batch_size, max_input_len=longest, max_output_len=max_new_tokens, dtype=td,
+                               kv_cache_bits=int(kv_bits)),
         max_step_tokens=max_step_tokens)
     gen = GenerationConfig(max_new_tokens=max_new_tokens, do_sample=temperature > 0, temperature=max(temperature, 1e-5),
                            top_k=top_k, top_p=top_p)

@@ -19,6 +19,9 @@ class InferenceConfig:
     # capture the decode step in a hipGraph (one graph per batch size):
     # removes per-layer launch gaps in the latency-bound decode loop
     use_hip_graph: bool = False
+    # paged caches of the Llama family: 16 keeps keys and values in the model's type, 4 in 4 bits (ops/cache_4bit.py: 17/32 byte a
+    # number; heads of 64, 128 or 256 channels, pages of 16 tokens and more)
+    kv_cache_bits: int = 16
 
     @property
     def max_seq_len(self) -> int:

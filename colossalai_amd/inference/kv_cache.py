@@ -31,6 +31,7 @@ class KVCacheManager:
         layer_sources: Optional[List[Optional[int]]] = None,
         layer_summaries: Optional[List[Optional[int]]] = None,
         layer_key_factors: Optional[List[bool]] = None,
+        bits: int = 16,
     ):
         """``layer_shapes`` (optional) gives each layer its own
         ``(kv_heads, key_dim, value_dim)`` (or ``(key_heads, key_dim, value_dim,
@@ -51,8 +52,14 @@ class KVCacheManager:
         ``layer_key_factors`` (optional) marks the layers that keep one float32 number per
         token and key head beside the key (keys normed on reading): ``k_factors[i]``
         ``[num_blocks, block_size, Hkv]``, addressed like the keys. A layer whose values
-        are its keys has a value size of 0; its attention reads ``k_pools[i]`` for both."""
+        are its keys has a value size of 0; its attention reads ``k_pools[i]`` for both. ``bits=4`` keeps the keys and values of
+        equal layers as 4-bit pools (``ops.kv4_pool``), which ``ops.paged_kv_append`` fills and ``ops.paged_attention_4bit`` reads."""
         assert block_size & (block_size - 1) == 0, "block_size must be a power of two"
+        if bits not in (4, 16):
+            raise ValueError(f"a cache keeps 16 bits (the model's type) or 4, got {bits}")
+        if bits == 4 and any(x is not None for x in (layer_shapes, layer_sources, layer_summaries, layer_key_factors)):
+            raise ValueError("4-bit caches are for layers of one kind")
+        self.bits, self.head_dim = bits, head_dim
         self.num_layers = num_layers
         self.block_size = block_size
         self.num_blocks = num_blocks
@@ -61,14 +68,13 @@ class KVCacheManager:
             layer_shapes = [(num_kv_heads, head_dim, head_dim)] * num_layers
         assert len(layer_shapes) == num_layers
         self.layer_shapes = list(layer_shapes)
-        self.k_pools = [
-            None if s is None else torch.zeros(num_blocks, block_size, s[0], s[1], device=self.device, dtype=dtype)
-            for s in layer_shapes
-        ]
-        self.v_pools = [
-            None if s is None else torch.zeros(num_blocks, block_size, s[-1] if len(s) > 3 else s[0], s[2], device=self.device, dtype=dtype)
-            for s in layer_shapes
-        ]
+        if bits == 4:
+            from ..ops.cache_4bit import kv4_pool
+
+            self.k_pools, self.v_pools = ([kv4_pool(num_blocks, block_size, num_kv_heads, head_dim, self.device) for _ in range(num_layers)]
+                                          for _ in range(2))
+        else:
+            self._make_pools(layer_shapes, dtype)
         self.layer_sources = list(layer_sources) if layer_sources is not None else [None] * num_layers
         assert len(self.layer_sources) == num_layers
         for i, src in enumerate(self.layer_sources):
@@ -98,6 +104,16 @@ class KVCacheManager:
                                                 dtype=torch.float32)
         self._free: List[int] = list(range(num_blocks - 1, -1, -1))
         self._tables: Dict[int, List[int]] = {}  # seq id -> block ids
+
+    def _make_pools(self, layer_shapes, dtype) -> None:
+        self.k_pools = [
+            None if s is None else torch.zeros(self.num_blocks, self.block_size, s[0], s[1], device=self.device, dtype=dtype)
+            for s in layer_shapes
+        ]
+        self.v_pools = [
+            None if s is None else torch.zeros(self.num_blocks, self.block_size, s[-1] if len(s) > 3 else s[0], s[2], device=self.device, dtype=dtype)
+            for s in layer_shapes
+        ]
 
     # ------------------------------------------------------------- accounting
     @property
@@ -141,8 +157,13 @@ class KVCacheManager:
         return bt
 
     # ---------------------------------------------------------------- writes
+    def _plain(self) -> None:
+        if self.bits == 4:
+            raise ValueError("a 4-bit cache is written by ops.paged_kv_append")
+
     def write_prefill(self, layer: int, seq_id: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """k/v [S, Hkv, D] for one sequence's prompt."""
+        self._plain()
         S = k.shape[0]
         bs = self.block_size
         table = self._tables[seq_id]
@@ -153,6 +174,7 @@ class KVCacheManager:
 
     def write_token(self, layer: int, seq_id: int, pos: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """k/v [Hkv, D] for the token at position pos."""
+        self._plain()
         bs = self.block_size
         blk = self._tables[seq_id][pos // bs]
         self.k_pools[layer][blk, pos % bs] = k
@@ -162,6 +184,11 @@ class KVCacheManager:
     def gather_contiguous(self, layer: int, seq_id: int, length: int):
         """CPU/reference path: materialize [length, Hkv, D] K and V."""
         table = self._tables[seq_id]
+        if self.bits == 4:
+            from ..ops.cache_4bit import kv4_read
+
+            rows = [table[p // self.block_size] * self.block_size + p % self.block_size for p in range(length)]
+            return kv4_read(self.k_pools[layer], self.v_pools[layer], torch.tensor(rows, dtype=torch.int32, device=self.device), self.head_dim)
         nb = self.blocks_needed(length)
         idx = torch.tensor(table[:nb], dtype=torch.long, device=self.device)
         k = self.k_pools[layer][idx].reshape(-1, *self.k_pools[layer].shape[2:])[:length]

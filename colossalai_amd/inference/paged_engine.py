@@ -9,6 +9,10 @@ Short requests retire and free their blocks immediately; long prompts
 stream in the moment blocks are available — throughput is bounded by the
 8 TB/s KV stream, not by the longest member of a static batch.
 
+Llama-family models whose query and key heads are normed, and caches in 4 bits (``kv_cache_bits=4``), take
+the same steps with their tokens packed: ``paged_kv_append`` norms, rotates and writes them, and
+attention reads the cache (``paged_attention`` / ``paged_attention_4bit``).
+
 Models that declare ``serves_ragged`` (hybrids of paged attention and
 fixed-size recurrent state) run through one *ragged* step instead:
 ``run_ragged`` takes any mix of prompt portions and single decode tokens,
@@ -55,6 +59,8 @@ class ContinuousBatchEngine:
         self.max_step_tokens = max_step_tokens
         self._gen = GenerationConfig()
         if self.ragged:
+            if self.config.kv_cache_bits != 16:
+                raise ValueError("4-bit caches are served for the Llama family")
             self.dtype = model.act_dtype
             shapes = model.kv_layer_shapes()
             sources = model.kv_layer_sources() if hasattr(model, "kv_layer_sources") else None
@@ -73,7 +79,10 @@ class ContinuousBatchEngine:
         attn0 = model.model.layers[0].self_attn
         self.kv = KVCacheManager(cfg.num_hidden_layers, attn0.num_kv_heads, attn0.head_dim,
                                  num_blocks=num_blocks, block_size=block_size,
-                                 device=self.device, dtype=self.dtype)
+                                 device=self.device, dtype=self.dtype, bits=self.config.kv_cache_bits)
+        self.packed = self.kv.bits == 4 or getattr(attn0, "qk_norm", False)
+        if self.kv.bits == 4 and torch.device(self.device).type == "cuda" and self.dtype != torch.bfloat16:
+            raise ValueError(f"a 4-bit cache on a GPU serves bfloat16 models, got {self.dtype}")
         self.rm = RequestManager(self.kv, max_batch_size=self.config.max_batch_size)
         self._gen = GenerationConfig()
 
@@ -185,6 +194,27 @@ class ContinuousBatchEngine:
             hidden = hidden.gather(1, gather)
         return self.model.lm_head(hidden[:, -1]).float()
 
+    def _forward_packed(self, items) -> torch.Tensor:
+        """``items`` is ``[(seq_id, new tokens, tokens in the cache)]``; the logits of each sequence's last token, float32."""
+        from ..ops import fused_add_rms_norm, rms_norm
+
+        m = self.model.model
+        batch = RaggedBatch.build([len(t) for _, t, _ in items], [s for _, _, s in items], list(range(len(items))), self.device,
+                                  [self.kv.table(i) for i, _, _ in items], self.kv.block_size, ordered=True)
+        flat = [t for _, tokens, _ in items for t in tokens]
+        ids, ends = to_device(flat + [n - 1 for n in batch.cu_host[1:]], torch.long, self.device, ordered=True).split([len(flat), len(items)])
+        table = m.rope_table(self.device)
+        residual = m.embed_tokens(ids[None])
+        hidden = rms_norm(residual, m.layers[0].input_layernorm_weight, m.eps)
+        n = len(m.layers)
+        for i, layer in enumerate(m.layers):
+            attn_out = layer.self_attn.forward_ragged(hidden, table, self.kv, i, batch)
+            hidden, residual = fused_add_rms_norm(attn_out, residual, layer.post_attention_layernorm_weight, m.eps)
+            mlp_out = layer.mlp(hidden)
+            next_w = m.layers[i + 1].input_layernorm_weight if i + 1 < n else m.norm_weight
+            hidden, residual = fused_add_rms_norm(mlp_out, residual, next_w, m.eps)
+        return self.model.lm_head(hidden[0, ends]).float()
+
     # ------------------------------------------------------------------ step
     @torch.inference_mode()
     def step(self) -> Dict[int, List[int]]:
@@ -196,6 +226,8 @@ class ContinuousBatchEngine:
         finished: Dict[int, List[int]] = {}
 
         admitted = self.rm.schedule()
+        if self.packed:
+            return self._step_packed(admitted)
         if admitted:
             prompts = [r.prompt for r in admitted]
             lens = torch.tensor([len(p) for p in prompts], device=self.device, dtype=torch.int32)
@@ -224,6 +256,25 @@ class ContinuousBatchEngine:
                 self.rm.append_token(r, int(tokens[i]), cfg.eos_token_id, cfg.max_seq_len)
                 if r.status.value == "finished":
                     finished[r.request_id] = r.tokens
+        return finished
+
+    def _step_packed(self, admitted) -> Dict[int, List[int]]:
+        """``step()`` with packed tokens: the prompts of the requests admitted, then one token of every running request."""
+        gen, cfg = self._gen, self.config
+        finished: Dict[int, List[int]] = {}
+
+        def advance(requests, items):
+            tokens = LLMEngine._sample(self._forward_packed(items), gen).tolist()
+            for r, token in zip(requests, tokens):
+                self.rm.append_token(r, int(token), cfg.eos_token_id, cfg.max_seq_len)
+                if r.status.value == "finished":
+                    finished[r.request_id] = r.tokens
+
+        if admitted:
+            advance(admitted, [(r.request_id, r.prompt, 0) for r in admitted])
+        running = list(self.rm.running)
+        if running:
+            advance(running, [(r.request_id, r.tokens[-1:], r.seq_len - 1) for r in running])
         return finished
 
     # ----------------------------------------------------------- convenience

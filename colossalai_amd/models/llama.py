@@ -49,6 +49,8 @@ class LlamaConfig:
     gradient_checkpointing: bool = False
     attention_bias: bool = False  # Qwen2-style qkv bias
     qk_norm: bool = False  # Qwen3-style per-head RMSNorm on q/k before RoPE
+    # the norms and the rotation in one pass over the projection (ops.qkv_norm_rope), which rounds once where the separate steps round twice
+    fused_qk_norm: bool = False
     head_dim_override: Optional[int] = None  # Qwen3 decouples head_dim from hidden/heads
     # GLM-4-style rope: rotate-every-two on the first (factor*head_dim) dims
     partial_interleaved_rotary_factor: float = 0.0
@@ -132,6 +134,7 @@ class LlamaAttention(nn.Module):
         self.o_proj = nn.Linear(Hq * D, cfg.hidden_size, bias=False)
         self.scale = 1.0 / math.sqrt(D)
         self.qk_norm = cfg.qk_norm
+        self.fused_qk_norm = cfg.fused_qk_norm
         self.pir_factor = cfg.partial_interleaved_rotary_factor
         self.rope_theta = cfg.rope_theta
         if cfg.qk_norm:
@@ -238,6 +241,13 @@ class LlamaAttention(nn.Module):
 
                 attn = attention_ref(q, k, v, causal=True, scale=self.scale, upcast=False)
             return project(self.o_proj, attn.reshape(B, S, Hq * D))
+        if self.qk_norm and self.fused_qk_norm:
+            from ..ops import flash_attention, qkv_norm_rope
+
+            q, k, v = qkv_norm_rope(qkv, self.q_norm_weight, self.k_norm_weight, rope_table, self.num_heads, self.num_kv_heads,
+                                    eps=self.norm_eps)
+            attn = flash_attention(q, k, v, causal=True, scale=self.scale, seqlens=seqlens)
+            return project(self.o_proj, attn.reshape(B, qkv.shape[1], -1))
         if self.qk_norm:
             # Qwen3: per-head RMSNorm on q/k before RoPE — unpack, norm,
             # rope, flash (the packed fused path skips the norm)
@@ -382,6 +392,23 @@ class LlamaAttention(nn.Module):
                                               causal=False, scale=self.scale))
                 out = torch.cat(outs, dim=0)
         return self.o_proj(out.reshape(B, S, -1))
+
+
+    def forward_ragged(self, hidden, rope_table, kv, layer_idx, batch):
+        """Attention of one step's tokens [1, N, hidden] (prompts, single tokens or both: ``batch`` is their ``RaggedBatch``) over a paged
+        cache, which takes their keys and values first. Norms of query and key heads, and caches in 4 bits, are served here."""
+        from ..ops.cache_4bit import paged_attention_4bit, paged_kv_append
+        from ..ops.paged_attention import paged_attention
+
+        if self.pir_factor != 0:
+            raise NotImplementedError("partial interleaved rotary heads are not served from this path")
+        N, Hq, Hkv, D = hidden.shape[1], self.num_heads, self.num_kv_heads, self.head_dim
+        q, k, v = self.qkv_proj(hidden).view(N, Hq + 2 * Hkv, D).split([Hq, Hkv, Hkv], 1)
+        norms = (self.q_norm_weight, self.k_norm_weight, self.norm_eps) if self.qk_norm else (None, None, 0.0)
+        kpool, vpool = kv.k_pools[layer_idx], kv.v_pools[layer_idx]
+        q = paged_kv_append(q, k, v, kpool, vpool, batch.kv_rows, batch.positions, rope_table, *norms)
+        attend = paged_attention_4bit if kv.bits == 4 else paged_attention
+        return self.o_proj(attend(q, kpool, vpool, batch, self.scale).reshape(1, N, Hq * D))
 
 
 class LlamaMLP(nn.Module):
