@@ -84,249 +84,88 @@ DEV_INLINE void unrolled(F f) {
   [&]<int... I>(std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>()), ...); }(std::make_integer_sequence<int, N>());
 }
 
+// A wave's rows: 16 RT of its tile, from `row0` on. A lane has a row of each 16 as its column.
 template <int D, int RT>
-__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attention_4bit_kernel(Attend a) {
-  constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;   // rows, products of a tile's scores, tiles of channels
-  __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
-  float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
-  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
-  const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
-  const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
-  const int per_token = min(a.group, R);
-  const int p0 = a.positions[t0], p1 = a.positions[t1 - 1];
-
-  // rows: queries, positions, places
+struct Rows {
+  static constexpr int KF = D / 32, VF = D / 16;   // products of a tile's scores, tiles of channels
   bf16x8_v q[RT][KF];
   int pos[RT], tok[RT], head[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = rt * 16 + n, in = sub * R + r % per_token;
-    tok[rt] = t0 + r / per_token;
-    const bool real = tok[rt] < t1 && in < a.group;
-    head[rt] = real ? g * a.group + in : -1;
-    pos[rt] = real ? a.positions[tok[rt]] : p1;
-    const bf16s* from = a.q + (real ? tok[rt] : t0) * a.q_stride + (long)(real ? head[rt] : g * a.group) * D + kg * (D / 4);
-#pragma unroll
-    for (int f = 0; f < KF; ++f) q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
-  }
-
-  const int* table = a.tables + (long)seq * a.width;
-  const float scale = a.scale * LOG2E4;
-
-  // a tile behind the end is its last one again: hidden by its places
-  auto look = [&](int (&pages)[2], int step) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) pages[h] = table[min(step * STEP + h * TILE, p1) >> a.page_shift];
-  };
-  auto load = [&](Raw<D>& w, int step, const int (&pages)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = min(step * STEP + h * TILE, p1), page = pages[h];
-      w.bad[h] = (unsigned)page >= (unsigned long)a.pages;
-      const long base = (long)(w.bad[h] ? 0 : page) * a.page_stride + (long)g * a.head_bytes +
-                        (long)((at & ((1 << a.page_shift) - 1)) / TILE) * Tile4<D>::BYTES;
-      const unsigned char *kt = a.kpool + base, *vt = a.vpool + base;
-      load_words(w.k[h], kt + n * (D / 2) + kg * (D / 8));
-      if constexpr (D == 256) w.ks[h] = *reinterpret_cast<const unsigned short*>(kt + Tile4<D>::key_scale(n, 2 * kg));
-      else w.ks[h] = kt[Tile4<D>::key_scale(n, D == 128 ? kg : kg >> 1)];
-      load_words(w.v[h], vt + (kg * 16 + n) * (D / 8));
-      w.vs[h] = *reinterpret_cast<const unsigned int*>(vt + Tile4<D>::value_scale(kg * 4, n * (D / 16) / 32));
-    }
-  };
-
   f32x4 o[RT][VF];
-  float m[RT], l[RT];
+  float2v state[RT];   // the reference, and the sum of the weights
+
+  // R: rows of the tile; p_last: the position of its last token
+  DEV_INLINE void start(const Attend& a, int R, int row0, int g, int sub, int t0, int t1, int p_last, int n, int kg) {
+    const int per_token = min(a.group, R);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = -INFINITY;
-    l[rt] = 0.0f;
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + rt * 16 + n, in = sub * R + r % per_token;
+      tok[rt] = t0 + r / per_token;
+      const bool real = tok[rt] < t1 && in < a.group;
+      head[rt] = real ? g * a.group + in : -1;
+      pos[rt] = real ? a.positions[tok[rt]] : p_last;
+      const bf16s* from = a.q + (real ? tok[rt] : t0) * a.q_stride + (long)(real ? head[rt] : g * a.group) * D + kg * (D / 4);
 #pragma unroll
-    for (int f = 0; f < VF; ++f) o[rt][f] = f32x4{0, 0, 0, 0};
+      for (int f = 0; f < KF; ++f) q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
+      state[rt] = float2v{-INFINITY, 0.0f};
+#pragma unroll
+      for (int f = 0; f < VF; ++f) o[rt][f] = f32x4{0, 0, 0, 0};
+    }
   }
 
-  auto compute = [&](const Raw<D>& w, int step) {
-    const int j = step * STEP;
-    // whether some row does not see some key of the step
-    const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
-    f32x4 s[RT][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][h] = f32x4{0, 0, 0, 0};
-      const float ks = scale_of(w.ks[h] & 255u), ks2 = scale_of(D == 256 ? w.ks[h] >> 8 : w.ks[h] & 255u);
-#pragma unroll
-      for (int f = 0; f < KF; ++f) {
-        const float u = D == 256 && f >= 4 ? ks2 : ks;
-        const unsigned int x = w.k[h][f];
-        const bf16x8_v k = frag(two_numbers<0>(x, u), two_numbers<1>(x, u), two_numbers<2>(x, u), two_numbers<3>(x, u));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[rt][f], s[rt][h], 0, 0, 0);
-      }
-    }
-    unsigned int vs[2] = {w.vs[0], w.vs[1]};
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[rt][h] *= scale;
-    if (edge) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = j + h * TILE + kg * 4 + i;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const bool seen = key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window);
-            s[rt][h][i] = !seen ? -INFINITY : w.bad[h] ? __builtin_nanf("") : s[rt][h][i];
-          }
-          if (key > p1 || (a.window > 0 && p0 - key >= a.window)) vs[h] &= ~(255u << (8 * i));
-        }
-      // a value that is not finite goes to the rows that see it through their weights: a weight of 0 would not hide it from the others
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned long long odd = __ballot(((vs[h] >> (8 * i)) & 255u) == 255u);
-          if (odd == 0) continue;
-          if ((odd >> (16 * kg)) & 0xffffu) {
-            const int key = j + h * TILE + kg * 4 + i;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              if (key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window)) s[rt][h][i] = __builtin_nanf("");
-            vs[h] &= ~(255u << (8 * i));
-          }
-        }
-    }
-    bf16x8_v p[RT], rest[RT];
+  DEV_INLINE bool sees(const Attend& a, int rt, int key) const { return key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window); }
+
+  // weights of the scores (base 2) of S steps as the product's operands, and with REST what bfloat16 leaves of them
+  template <bool REST, int S>
+  DEV_INLINE void weigh(const f32x4 (&s)[RT][2 * S], bf16x8_v (&p)[RT][S], bf16x8_v (&rest)[RT][S]) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2 * S; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
-      if (__any(top > m[rt] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
-        const float next = fmaxf(m[rt], top), fall = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - next);
-        m[rt] = next;
-        l[rt] *= fall;
+      if (__any(top > state[rt][0] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
+        const float m = state[rt][0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        state[rt] = float2v{next, state[rt][1] * fall};
 #pragma unroll
         for (int f = 0; f < VF; ++f) o[rt][f] *= fall;
       }
-      const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
-      float e[8];
+      const float ref = state[rt][0] == -INFINITY ? 0.0f : state[rt][0];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int step = 0; step < S; ++step) {
+        float e[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[h * 4 + i] = __builtin_amdgcn_exp2f(s[rt][h][i] - ref);
-          l[rt] += e[h * 4 + i];
+        for (int i = 0; i < 8; ++i) {
+          e[i] = __builtin_amdgcn_exp2f(s[rt][2 * step + i / 4][i % 4] - ref);
+          state[rt][1] += e[i];
         }
-      const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
-      p[rt] = __builtin_bit_cast(bf16x8_v, w);
-      if constexpr (RT == 1) {
+        const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
+        p[rt][step] = __builtin_bit_cast(bf16x8_v, w);
+        if constexpr (REST) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-        rest[rt] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
-      }
-    }
-    float su[2][4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) su[h][i] = scale_of((vs[h] >> (8 * i)) & 255u);
-    unrolled<D / 32>([&](auto byte) {
-      constexpr int B = decltype(byte)::value;
-      unsigned int lo0[2], hi0[2], lo1[2], hi1[2];
-      value_words<D, B>(w.v[0], su[0], lo0, hi0);
-      value_words<D, B>(w.v[1], su[1], lo1, hi1);
-      const bf16x8_v lo = frag(lo0[0], lo0[1], lo1[0], lo1[1]), hi = frag(hi0[0], hi0[1], hi1[0], hi1[1]);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt], o[rt][2 * B], 0, 0, 0);
-        o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt], o[rt][2 * B + 1], 0, 0, 0);
-        if constexpr (RT == 1) {
-          o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt], o[rt][2 * B], 0, 0, 0);
-          o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt], o[rt][2 * B + 1], 0, 0, 0);
+          for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+          rest[rt][step] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
         }
       }
-    });
-  };
-
-  // the next step's codes are on their way while a step is worked on, and the page numbers of the one after it
-  int step = from + wid;
-  if (step < to) {
-    Raw<D> even, odd;
-    int pages[2];
-    look(pages, step);
-    load(even, step, pages);
-    look(pages, step + WAVES4);
-    while (true) {
-      if (step + WAVES4 < to) {
-        load(odd, step + WAVES4, pages);
-        look(pages, step + 2 * WAVES4);
-      }
-      compute(even, step);
-      if ((step += WAVES4) >= to) break;
-      if (step + WAVES4 < to) {
-        load(even, step + WAVES4, pages);
-        look(pages, step + 2 * WAVES4);
-      }
-      compute(odd, step);
-      if ((step += WAVES4) >= to) break;
     }
   }
 
-  // the waves' states meet: a common reference, then sums in pairs
+  // sums of the lanes that share a row
+  DEV_INLINE void sum_lanes() {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16);
-    l[rt] += __shfl_xor(l[rt], 32);
-    if (kg == 0) states[wid][rt * 16 + n] = float2v{m[rt], l[rt]};
-  }
-  __syncthreads();
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES4; ++w) top = fmaxf(top, states[w][rt * 16 + n][0]);
-#pragma unroll
-    for (int w = 0; w < WAVES4; ++w) {
-      const float2v x = states[w][rt * 16 + n];   // without a reference the sum is 0, or NaN, which stays
-      sum += x[0] == -INFINITY ? x[1] : x[1] * __builtin_amdgcn_exp2f(x[0] - top);
+    for (int rt = 0; rt < RT; ++rt) {
+      state[rt][1] += __shfl_xor(state[rt][1], 16);
+      state[rt][1] += __shfl_xor(state[rt][1], 32);
     }
-    const float mine = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - top);
-#pragma unroll
-    for (int f = 0; f < VF; ++f) o[rt][f] *= mine;
-    m[rt] = top;
-    l[rt] = sum;
   }
-  __syncthreads();
-#pragma unroll
-  for (int live = WAVES4 / 2; live > 0; live >>= 1) {
-    if (wid >= live && wid < 2 * live) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int f = 0; f < VF; ++f) lds[wid - live][rt * VF + f][lane] = o[rt][f];
-    }
-    __syncthreads();
-    if (wid < live) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int f = 0; f < VF; ++f) o[rt][f] += lds[wid][rt * VF + f][lane];
-    }
-    __syncthreads();
-  }
-  if (wid != 0) return;
-  if (slot < 0) {   // the only part
+
+  DEV_INLINE void store(const Attend& a, int kg) const {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (head[rt] < 0) continue;
-      const float inv = 1.0f / l[rt];
+      const float inv = 1.0f / state[rt][1];
       bf16s* to_row = a.out + ((long)tok[rt] * a.H + head[rt]) * D;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -338,29 +177,342 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
         for (int f = 0; f < VF / 2; f += 2) *reinterpret_cast<uint2*>(to_ch + f) = make_uint2(w[f], w[f + 1]);
       }
     }
-    return;
   }
-  // a part: rows' sums, then their references and weights
-  float* part = a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L));
+
+  // into a part of R rows: rows' sums, then their references and weights
+  DEV_INLINE void store_part(float* part, int R, int row0, int n, int kg) const {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (head[rt] < 0) continue;
+      const int r = row0 + rt * 16 + n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int f = 0; f < VF; f += 4)
+          *reinterpret_cast<float4v*>(part + (long)r * D + (kg * 4 + i) * VF + f) = float4v{o[rt][f][i], o[rt][f + 1][i], o[rt][f + 2][i], o[rt][f + 3][i]};
+      if (kg == 0) *reinterpret_cast<float2v*>(part + (long)R * D + r * 2) = state[rt];
+    }
+  }
+};
+
+// Where a step's codes come from: the pages of a sequence, for one key head.
+template <int D>
+struct Source {
+  const int* table;
+  int p_last, g;
+  // a tile behind the end is its last one again: hidden by its places
+  DEV_INLINE void look(const Attend& a, int (&pages)[2], int step) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) pages[h] = table[min(step * STEP + h * TILE, p_last) >> a.page_shift];
+  }
+  DEV_INLINE void load(const Attend& a, Raw<D>& w, int step, const int (&pages)[2], int n, int kg) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = min(step * STEP + h * TILE, p_last), page = pages[h];
+      w.bad[h] = (unsigned)page >= (unsigned long)a.pages;
+      const long base = (long)(w.bad[h] ? 0 : page) * a.page_stride + (long)g * a.head_bytes +
+                        (long)((at & ((1 << a.page_shift) - 1)) / TILE) * Tile4<D>::BYTES;
+      const unsigned char *kt = a.kpool + base, *vt = a.vpool + base;
+      load_words(w.k[h], kt + n * (D / 2) + kg * (D / 8));
+      if constexpr (D == 256) w.ks[h] = *reinterpret_cast<const unsigned short*>(kt + Tile4<D>::key_scale(n, 2 * kg));
+      else w.ks[h] = kt[Tile4<D>::key_scale(n, D == 128 ? kg : kg >> 1)];
+      load_words(w.v[h], vt + (kg * 16 + n) * (D / 8));
+      w.vs[h] = *reinterpret_cast<const unsigned int*>(vt + Tile4<D>::value_scale(kg * 4, n * (D / 16) / 32));
+    }
+  }
+};
+
+// Fragment f of a tile's keys, and the two of byte B of a step's values.
+template <int D>
+DEV_INLINE bf16x8_v key_frag(const Raw<D>& w, int h, int f) {
+  const float u = scale_of(D == 256 && f >= 4 ? w.ks[h] >> 8 : w.ks[h] & 255u);
+  const unsigned int x = w.k[h][f];
+  return frag(two_numbers<0>(x, u), two_numbers<1>(x, u), two_numbers<2>(x, u), two_numbers<3>(x, u));
+}
+template <int D, int B>
+DEV_INLINE void value_frags(const Raw<D>& w, const float (&su)[2][4], bf16x8_v& lo, bf16x8_v& hi) {
+  unsigned int lo0[2], hi0[2], lo1[2], hi1[2];
+  value_words<D, B>(w.v[0], su[0], lo0, hi0);
+  value_words<D, B>(w.v[1], su[1], lo1, hi1);
+  lo = frag(lo0[0], lo0[1], lo1[0], lo1[1]);
+  hi = frag(hi0[0], hi0[1], hi1[0], hi1[1]);
+}
+
+// What a step's values are to be taken at: 0 for keys that no row from position p_first to p_last sees. `odd`: of the lane's keys
+// (4 h + i) those that show NaN to the rows that see them, as their page or their value's scale is none: a weight of 0 would not hide such a
+// value, so that it is taken as 0 too and goes to the rows through their scores.
+template <int D>
+DEV_INLINE unsigned int value_scales(const Attend& a, const Raw<D>& w, float (&su)[2][4], int step, int p_first, int p_last, int kg, bool look) {
+  unsigned int odd = 0, vs[2] = {w.vs[0], w.vs[1]};
+  if (look) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = step * STEP + h * TILE + kg * 4 + i;
+        if (key > p_last || (a.window > 0 && p_first - key >= a.window)) vs[h] &= ~(255u << (8 * i));
+      }
+    auto none = [](unsigned int v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & v & 0x80808080u; };   // the bytes of 255
+    if (__any((none(vs[0]) | none(vs[1])) != 0) || w.bad[0] || w.bad[1]) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned long long lanes = __ballot(((vs[h] >> (8 * i)) & 255u) == 255u);
+          if (!w.bad[h] && ((lanes >> (16 * kg)) & 0xffffu) == 0) continue;
+          odd |= 1u << (4 * h + i);   // where it is not seen at all, it does not show either
+          vs[h] &= ~(255u << (8 * i));
+        }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) su[h][i] = scale_of((vs[h] >> (8 * i)) & 255u);
+  return odd;
+}
+
+// Few rows: a block has a tile of 16 RT rows and its waves take its steps in turn.
+template <int D, int RT>
+__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attention_4bit_kernel(Attend a) {
+  constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;
+  __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
+  float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
+  const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
+  const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
+  const int p0 = a.positions[t0], p1 = a.positions[t1 - 1];
+  Rows<D, RT> rows;
+  rows.start(a, R, 0, g, sub, t0, t1, p1, n, kg);
+  const Source<D> source = {a.tables + (long)seq * a.width, p1, g};
+  const float scale = a.scale * LOG2E4;
+
+  auto compute = [&](const Raw<D>& w, int step) {
+    const int j = step * STEP;
+    // whether some row does not see some key of the step
+    const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
+    f32x4 s[RT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int f = 0; f < KF; ++f) {
+        const bf16x8_v k = key_frag(w, h, f);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, rows.q[rt][f], s[rt][h], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[rt][h] *= scale;
+    float su[2][4];
+    const unsigned int odd = value_scales(a, w, su, step, p0, p1, kg, edge);
+    if (edge) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            s[rt][h][i] = !rows.sees(a, rt, j + h * TILE + kg * 4 + i) ? -INFINITY : odd >> (4 * h + i) & 1 ? __builtin_nanf("") : s[rt][h][i];
+    }
+    bf16x8_v p[RT][1], rest[RT][1];
+    rows.template weigh<RT == 1, 1>(s, p, rest);
+    unrolled<D / 32>([&](auto byte) {
+      constexpr int B = decltype(byte)::value;
+      bf16x8_v lo, hi;
+      value_frags<D, B>(w, su, lo, hi);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt][0], rows.o[rt][2 * B], 0, 0, 0);
+        rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt][0], rows.o[rt][2 * B + 1], 0, 0, 0);
+        if constexpr (RT == 1) {
+          rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt][0], rows.o[rt][2 * B], 0, 0, 0);
+          rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt][0], rows.o[rt][2 * B + 1], 0, 0, 0);
+        }
+      }
+    });
+  };
+
+  // the next step's codes are on their way while a step is worked on, and the page numbers of the one after it
+  int step = from + wid;
+  if (step < to) {
+    Raw<D> even, odd;
+    int pages[2];
+    source.look(a, pages, step);
+    source.load(a, even, step, pages, n, kg);
+    source.look(a, pages, step + WAVES4);
+    while (true) {
+      if (step + WAVES4 < to) {
+        source.load(a, odd, step + WAVES4, pages, n, kg);
+        source.look(a, pages, step + 2 * WAVES4);
+      }
+      compute(even, step);
+      if ((step += WAVES4) >= to) break;
+      if (step + WAVES4 < to) {
+        source.load(a, even, step + WAVES4, pages, n, kg);
+        source.look(a, pages, step + 2 * WAVES4);
+      }
+      compute(odd, step);
+      if ((step += WAVES4) >= to) break;
+    }
+  }
+
+  // the waves' states meet: a common reference, then sums in pairs
+  rows.sum_lanes();
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+    if (kg == 0) states[wid][rt * 16 + n] = rows.state[rt];
+  __syncthreads();
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    if (head[rt] < 0) continue;
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int w = 0; w < WAVES4; ++w) top = fmaxf(top, states[w][rt * 16 + n][0]);
 #pragma unroll
-      for (int f = 0; f < VF; f += 4)
-        *reinterpret_cast<float4v*>(part + (rt * 16 + n) * D + (kg * 4 + i) * VF + f) = float4v{o[rt][f][i], o[rt][f + 1][i], o[rt][f + 2][i], o[rt][f + 3][i]};
-    if (kg == 0) *reinterpret_cast<float2v*>(part + (long)R * D + (rt * 16 + n) * 2) = float2v{m[rt], l[rt]};
+    for (int w = 0; w < WAVES4; ++w) {
+      const float2v x = states[w][rt * 16 + n];   // without a reference the sum is 0, or NaN, which stays
+      sum += x[0] == -INFINITY ? x[1] : x[1] * __builtin_amdgcn_exp2f(x[0] - top);
+    }
+    const float mine = rows.state[rt][0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rows.state[rt][0] - top);
+#pragma unroll
+    for (int f = 0; f < VF; ++f) rows.o[rt][f] *= mine;
+    rows.state[rt] = float2v{top, sum};
   }
+  __syncthreads();
+#pragma unroll
+  for (int live = WAVES4 / 2; live > 0; live >>= 1) {
+    if (wid >= live && wid < 2 * live) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int f = 0; f < VF; ++f) lds[wid - live][rt * VF + f][lane] = rows.o[rt][f];
+    }
+    __syncthreads();
+    if (wid < live) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int f = 0; f < VF; ++f) rows.o[rt][f] += lds[wid][rt * VF + f][lane];
+    }
+    __syncthreads();
+  }
+  if (wid != 0) return;
+  if (slot < 0) rows.store(a, kg);   // the only part
+  else rows.store_part(a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L)), R, 0, n, kg);
+}
+
+// Many rows: a block has a tile of 32 WAVES4 rows, 32 a wave, and all its waves take the same steps. Each makes one of WAVES4 steps' codes into
+// fragments in LDS, which the others read: the conversions, half of what a wave of the other form issues, are then done once for the block.
+template <int D>
+__global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(Attend a) {
+  constexpr int RT = 2, R = 16 * RT * WAVES4, KF = D / 32, VF = D / 16;
+  __shared__ uint4v frags[WAVES4][2 * KF + VF][64];
+  __shared__ unsigned int odds[WAVES4][4];
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
+  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
+  const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
+  const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
+  const int p0 = a.positions[t0], p1 = a.positions[t1 - 1], per_token = min(a.group, R), row0 = wid * 16 * RT;
+  Rows<D, RT> rows;
+  rows.start(a, R, row0, g, sub, t0, t1, p1, n, kg);
+  // of the wave's own rows; without any it just works for the others
+  const int mine0 = p0 + row0 / per_token, mine1 = min(p1, p0 + (row0 + 16 * RT - 1) / per_token);
+  const Source<D> source = {a.tables + (long)seq * a.width, p1, g};
+  const float scale = a.scale * LOG2E4;
+  Raw<D> w;
+  int pages[2];
+  source.look(a, pages, from + wid);
+  source.load(a, w, from + wid, pages, n, kg);
+  for (int base = from; base < to; base += WAVES4) {
+    __syncthreads();   // the fragments before have been used
+    if (base + wid < to) {
+      const int step = base + wid, j = step * STEP;
+      const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < KF; ++f) frags[wid][h * KF + f][lane] = __builtin_bit_cast(uint4v, key_frag(w, h, f));
+      float su[2][4];
+      const unsigned int odd = value_scales(a, w, su, step, p0, p1, kg, edge);
+      if (n == 0) odds[wid][kg] = odd;
+      unrolled<D / 32>([&](auto byte) {
+        constexpr int B = decltype(byte)::value;
+        bf16x8_v lo, hi;
+        value_frags<D, B>(w, su, lo, hi);
+        frags[wid][2 * KF + 2 * B][lane] = __builtin_bit_cast(uint4v, lo);
+        frags[wid][2 * KF + 2 * B + 1][lane] = __builtin_bit_cast(uint4v, hi);
+      });
+      if (step + WAVES4 < to) {
+        source.look(a, pages, step + WAVES4);
+        source.load(a, w, step + WAVES4, pages, n, kg);
+      }
+    }
+    __syncthreads();
+    const int ready = min(WAVES4, to - base);
+    // S of the steps that lie ready, from the i-th on
+    auto compute = [&](auto steps, int i) {
+      constexpr int S = decltype(steps)::value;
+      const int j = (base + i) * STEP, end = j + S * STEP - 1;
+      if (mine0 > mine1 || j > mine1 || (a.window > 0 && mine0 - end >= a.window)) return;   // nothing to see
+      f32x4 s[RT][2 * S];
+#pragma unroll
+      for (int h = 0; h < 2 * S; ++h) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int f = 0; f < KF; ++f) {
+          const bf16x8_v k = __builtin_bit_cast(bf16x8_v, frags[i + h / 2][h % 2 * KF + f][lane]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, rows.q[rt][f], s[rt][h], 0, 0, 0);
+        }
+      }
+      unsigned int odd = 0;
+#pragma unroll
+      for (int h = 0; h < S; ++h) odd |= odds[i + h][kg] << (8 * h);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int h = 0; h < 2 * S; ++h) s[rt][h] *= scale;
+      if (end > mine0 || (a.window > 0 && mine1 - j >= a.window) || __any(odd != 0)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int h = 0; h < 2 * S; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[rt][h][e] = !rows.sees(a, rt, j + h * TILE + kg * 4 + e) ? -INFINITY : odd >> (4 * h + e) & 1 ? __builtin_nanf("") : s[rt][h][e];
+      }
+      bf16x8_v p[RT][S], rest[RT][S];
+      rows.template weigh<false, S>(s, p, rest);
+#pragma unroll
+      for (int h = 0; h < S; ++h)
+#pragma unroll
+        for (int f = 0; f < VF; ++f) {
+          const bf16x8_v v = __builtin_bit_cast(bf16x8_v, frags[i + h][2 * KF + f][lane]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) rows.o[rt][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rt][h], rows.o[rt][f], 0, 0, 0);
+        }
+    };
+    int i = 0;
+    for (; i + 2 <= ready; i += 2) compute(std::integral_constant<int, 2>(), i);
+    if (i < ready) compute(std::integral_constant<int, 1>(), i);
+  }
+  rows.sum_lanes();
+  if (slot < 0) rows.store(a, kg);
+  else rows.store_part(a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L)), R, row0, n, kg);
 }
 
 // Puts the parts of a tile's rows together: a block takes 512 / D rows, eight channels a lane; its waves take eight parts each at a time, so that
 // few round trips to memory follow each other, and meet in LDS.
 constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
 
-template <int D, int RT>
+template <int D, int R>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_4bit_join_kernel(Attend a) {
-  constexpr int R = 16 * RT, LANES = D / 8;
+  constexpr int LANES = D / 8;
   __shared__ float lds[JOIN_WAVES][10][64];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, c = lane % LANES * 8, r = blockIdx.y * (64 / LANES) + lane / LANES;
   const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
@@ -428,26 +580,29 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_4bit_join_kernel(At
   store8(a.out + ((long)tok * a.H + g * a.group + in) * D + c, o);
 }
 
-template <int D, int RT>
+// R: rows of a tile, 16 or 32 for one wave's, 32 WAVES4 for the waves of a block
+template <int D, int R>
 void launch(Attend a, long items, long slots, long joins, const at::Tensor& like) {
-  a.subs = (a.group + 16 * RT - 1) / (16 * RT);
+  a.subs = (a.group + R - 1) / R;
   const long heads = (long)a.G * a.subs;
   at::Tensor parts;
   if (joins > 0) {
-    parts = at::empty({slots * heads * 16 * RT * (D + 2)}, like.options().dtype(at::kFloat));
+    parts = at::empty({slots * heads * R * (D + 2)}, like.options().dtype(at::kFloat));
     a.parts = parts.data_ptr<float>();
   }
-  hipLaunchKernelGGL((attention_4bit_kernel<D, RT>), dim3((unsigned)(items * heads)), dim3(64 * WAVES4), 0, stream(), a);
+  const dim3 grid((unsigned)(items * heads)), block(64 * WAVES4);
+  if constexpr (R == 32 * WAVES4) hipLaunchKernelGGL((attention_4bit_shared_kernel<D>), grid, block, 0, stream(), a);
+  else hipLaunchKernelGGL((attention_4bit_kernel<D, R / 16>), grid, block, 0, stream(), a);
   HIP_CHECK_LAST();
   if (joins > 0) {
-    hipLaunchKernelGGL((attention_4bit_join_kernel<D, RT>), dim3((unsigned)(joins * heads), 16 * RT * D / 512), dim3(64 * JOIN_WAVES), 0, stream(), a);
+    hipLaunchKernelGGL((attention_4bit_join_kernel<D, R>), dim3((unsigned)(joins * heads), R * D / 512), dim3(64 * JOIN_WAVES), 0, stream(), a);
     HIP_CHECK_LAST();
   }
 }
 
 }  // namespace
 
-// `plan`: of the tiles with at most 16 rows, then of those with at most 32, what a block does, (sequence, first token, end token, first step,
+// `plan`: of the tiles with at most 16 rows, then of those with at most 32, then of those with at most 128 (heads of up to 128 channels), what a block does, (sequence, first token, end token, first step,
 // end step, part or -1) for each, then the tiles that have parts, (first token, end token, first part, parts). `sizes`: of each kind the numbers of
 // both, and of parts.
 at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions,
@@ -464,8 +619,8 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   check_i32(block_tables, "block_tables");
   check_i32(plan, "plan");
   check_i32(positions, "positions");
-  TORCH_CHECK_VALUE(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 6 &&
-              plan.numel() == 6 * (sizes[0] + sizes[3]) + 4 * (sizes[1] + sizes[4]), who, "batch of other tokens");
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 9 &&
+              plan.numel() == 6 * (sizes[0] + sizes[3] + sizes[6]) + 4 * (sizes[1] + sizes[4] + sizes[7]), who, "batch of other tokens");
   for (const at::Tensor& t : {kpool, vpool, block_tables, positions, plan})
     TORCH_CHECK_VALUE(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
   const bool fits = q_in.stride(2) == 1 && q_in.stride(1) == D && q_in.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(q_in.data_ptr()) % 16 == 0;
@@ -493,14 +648,16 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   auto run = [&](auto size) {
     constexpr int DD = decltype(size)::value;
     const int* at = plan.data_ptr<int>();
-    for (int kind = 0; kind < 2; ++kind) {
+    for (int kind = 0; kind < 3; ++kind) {
       const long items = sizes[3 * kind], joins = sizes[3 * kind + 1], slots = sizes[3 * kind + 2];
       a.items = at;
       a.joins = at + 6 * items;
       at = a.joins + 4 * joins;
       if (items == 0) continue;
-      if (kind == 0) launch<DD, 1>(a, items, slots, joins, q);
-      else launch<DD, 2>(a, items, slots, joins, q);
+      if (kind == 0) launch<DD, 16>(a, items, slots, joins, q);
+      else if (kind == 1) launch<DD, 32>(a, items, slots, joins, q);
+      else if constexpr (DD <= 128) launch<DD, 32 * WAVES4>(a, items, slots, joins, q);
+      else TORCH_CHECK_VALUE(false, who, "tiles of 128 rows are for heads of up to 128 channels");
     }
   };
   if (D == 64) run(std::integral_constant<int, 64>());

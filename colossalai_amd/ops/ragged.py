@@ -12,6 +12,7 @@ else shares the step.
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from ._kernels import serving_kernels
@@ -57,6 +58,18 @@ def to_device(values: Sequence, dtype, device, ordered: bool = False) -> torch.T
         return torch.tensor(values, dtype=dtype, pin_memory=True).to(device, non_blocking=True)
 
     return copy() if ordered else complete(copy, device)
+
+
+def _share(steps, blocks_each: int, most: int, least: int) -> int:
+    """The longest part, in steps, that tiles of ``steps`` are cut into: where their blocks (`blocks_each` a part) leave some of the `most` that a
+    chip holds at once, the smallest parts that still are all at once, `least` steps at least; else none is cut."""
+    lo, hi = least, int(steps.max())
+    if len(steps) * blocks_each >= most:
+        return hi
+    while lo < hi:
+        mid = (lo + hi) // 2
+        lo, hi = (lo, mid) if int((-(-steps // mid)).sum()) * blocks_each <= most else (mid + 1, hi)
+    return hi
 
 
 @dataclass
@@ -139,58 +152,53 @@ class RaggedBatch:
             self._even[window, fewest] = (total / (tiles * most), int(most)) if tiles else (0.5, 0)
         return self._even[window, fewest]
 
-    def row_plan(self, group: int, heads: int, window: int = 0, blocks: Sequence[int] = (1024, 512), step: int = 32, least: int = 8):
+    def row_plan(self, group: int, heads: int, window: int = 0, blocks: Sequence[int] = (1024, 512, 512), step: int = 32, least: int = 8):
         """The work of an attention kernel whose block takes a tile of rows (the `group` query heads of a key head for some tokens) and a part of
         their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles have 16
-        rows where a sequence's new tokens are at most as many rows, or one token, else 32. A tile's keys are cut into even parts of at
-        least `least` steps, as many as the `blocks` that a chip holds at once (of tiles of 16 and of 32 rows) allow; `heads` blocks share a part.
-        Tiles with more keys come first. Built once per step and kind, shared by its layers."""
+        rows where a sequence's new tokens are at most as many rows, or one token, 128 where they are 96 and more, else 32. A tile's keys are cut
+        into even parts of at least `least` steps, as many as the `blocks` that a chip holds at once (of tiles of 16, 32 and 128 rows; 0: no
+        such tiles) allow; `heads` key heads have a block each for a part. Tiles with more keys come first. Built once per step
+        and kind, shared by its layers."""
         if self._rows is None:
             self._rows = {}
         key = group, heads, window, tuple(blocks)
         if key not in self._rows:
-            cu, start = torch.tensor(self.cu_host), torch.tensor(self.start_host)
+            cu, start = np.array(self.cu_host), np.array(self.start_host)
             new = cu[1:] - cu[:-1]
-            short = (new == 1) | (new * group <= 16)
+            few = (new == 1) | (new * group <= 16)
+            many = ~few & (new * group >= 96) & (blocks[2] > 0)
             parts, sizes = [], []
-            for rows, pick, most in ((16, short, blocks[0]), (32, ~short, blocks[1])):
-                seqs = pick.nonzero()[:, 0]
+            for rows, pick, most in ((16, few, blocks[0]), (32, ~few & ~many, blocks[1]), (128, many, blocks[2])):
+                seqs = np.flatnonzero(pick)
+                if not len(seqs):
+                    sizes += [0, 0, 0]
+                    continue
                 per = max(1, rows // group)
+                each_part = heads * -(-group // rows)  # blocks
                 tiles = (new[seqs] + per - 1) // per
-                of = seqs.repeat_interleave(tiles)
-                nth = torch.arange(len(of)) - (tiles.cumsum(0) - tiles).repeat_interleave(tiles)
-                t0 = cu[of] + nth * per
-                t1 = torch.minimum(t0 + per, cu[of + 1])
+                of = np.repeat(seqs, tiles)
+                t0 = cu[of] + (np.arange(len(of)) - np.repeat(tiles.cumsum() - tiles, tiles)) * per
+                t1 = np.minimum(t0 + per, cu[of + 1])
                 shift = start[of] - cu[of]
-                begin = (t0 + shift - window + 1).clamp(min=0) // step if window > 0 else torch.zeros_like(t0)
+                begin = np.maximum(t0 + shift - window + 1, 0) // step if window > 0 else np.zeros_like(t0)
                 steps = (t1 - 1 + shift) // step + 1 - begin
-                order = steps.argsort(descending=True, stable=True)
-                of, t0, t1, begin, steps = (x[order] for x in (of, t0, t1, begin, steps))
-                share = int(steps[0]) if len(steps) else 1
-                if 0 < len(steps) * heads < most:  # the smallest parts that the chip takes at once
-                    lo, hi = min(least, share), share
-                    while lo < hi:
-                        mid = (lo + hi) // 2
-                        if int(((steps + mid - 1) // mid).sum()) * heads <= most:
-                            hi = mid
-                        else:
-                            lo = mid + 1
-                    share = lo
-                count = (steps + share - 1) // share
-                each = (steps + count - 1) // count
-                count = (steps + each - 1) // each  # none is empty
-                many = count > 1
-                slots = torch.where(many, count, 0)
-                first = slots.cumsum(0) - slots
-                tile = torch.arange(len(of)).repeat_interleave(count)
-                part = torch.arange(len(tile)) - (count.cumsum(0) - count)[tile]
+                order = np.argsort(-steps, kind="stable")
+                of, t0, t1, begin, steps = of[order], t0[order], t1[order], begin[order], steps[order]
+                share = _share(steps, each_part, most, least)
+                count = -(-steps // share)
+                each = -(-steps // count)
+                count = -(-steps // each)  # none is empty
+                cut = count > 1
+                slots = count * cut
+                first = slots.cumsum() - slots
+                tile = np.repeat(np.arange(len(of)), count)
+                part = np.arange(len(tile)) - (count.cumsum() - count)[tile]
                 lo = begin[tile] + part * each[tile]
-                hi = torch.minimum(lo + each[tile], (begin + steps)[tile])
-                slot = torch.where(many[tile], first[tile] + part, -1)
-                parts += [torch.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1).flatten(),
-                          torch.stack([t0, t1, first, count], 1)[many].flatten()]
-                sizes += [len(tile), int(many.sum()), int(slots.sum())]
-            self._rows[key] = to_device(torch.cat(parts).tolist(), torch.int32, self.cu.device, self.ordered), sizes
+                hi = np.minimum(lo + each[tile], (begin + steps)[tile])
+                slot = np.where(cut[tile], first[tile] + part, -1)
+                parts += [np.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1).ravel(), np.stack([t0, t1, first, count], 1)[cut].ravel()]
+                sizes += [len(tile), int(cut.sum()), int(slots.sum())]
+            self._rows[key] = to_device(np.concatenate(parts).tolist(), torch.int32, self.cu.device, self.ordered), sizes
         return self._rows[key]
 
     @property
