@@ -508,7 +508,7 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
 
 // Puts the parts of a tile's rows together: a block takes 512 / D rows, eight channels a lane; its waves take eight parts each at a time, so that
 // few round trips to memory follow each other, and meet in LDS.
-constexpr int JOIN_WAVES = 4, AT_ONCE = 8;
+constexpr int JOIN_WAVES = 8, AT_ONCE = 8;
 
 template <int D, int R>
 __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_4bit_join_kernel(Attend a) {

@@ -19,6 +19,7 @@ from ._kernels import serving_kernels
 
 __all__ = ["RaggedBatch", "to_device"]
 
+_CUS = 256  # of a chip
 LISTED_TOKENS = 32  # up to here a step's per-token vectors are made on the host: a launch takes as long
 
 
@@ -155,9 +156,10 @@ class RaggedBatch:
     def row_plan(self, group: int, heads: int, window: int = 0, blocks: Sequence[int] = (1024, 512, 512), step: int = 32, least: int = 8):
         """The work of an attention kernel whose block takes a tile of rows (the `group` query heads of a key head for some tokens) and a part of
         their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles have 16
-        rows where a sequence's new tokens are at most as many rows, or one token, 128 where they are 96 and more, else 32. A tile's keys are cut
+        rows where a sequence's new tokens are at most as many rows, or one token (32 beside other tiles of 32, if they do not fill half the chip),
+        128 where they are 96 and more, else 32. A tile's keys are cut
         into even parts of at least `least` steps, as many as the `blocks` that a chip holds at once (of tiles of 16, 32 and 128 rows; 0: no
-        such tiles) allow; `heads` key heads have a block each for a part. Tiles with more keys come first. Built once per step
+        such tiles) allow; `heads` key heads have a block each for a part. Longer parts come first. Built once per step
         and kind, shared by its layers."""
         if self._rows is None:
             self._rows = {}
@@ -167,6 +169,9 @@ class RaggedBatch:
             new = cu[1:] - cu[:-1]
             few = (new == 1) | (new * group <= 16)
             many = ~few & (new * group >= 96) & (blocks[2] > 0)
+            if few.sum() * heads < blocks[0] // 2 and (~few & ~many).any():  # one launch: there is room beside the others
+                few[:] = False
+                many &= new > 1
             parts, sizes = [], []
             for rows, pick, most in ((16, few, blocks[0]), (32, ~few & ~many, blocks[1]), (128, many, blocks[2])):
                 seqs = np.flatnonzero(pick)
@@ -182,8 +187,6 @@ class RaggedBatch:
                 shift = start[of] - cu[of]
                 begin = np.maximum(t0 + shift - window + 1, 0) // step if window > 0 else np.zeros_like(t0)
                 steps = (t1 - 1 + shift) // step + 1 - begin
-                order = np.argsort(-steps, kind="stable")
-                of, t0, t1, begin, steps = of[order], t0[order], t1[order], begin[order], steps[order]
                 share = _share(steps, each_part, most, least)
                 count = -(-steps // share)
                 each = -(-steps // count)
@@ -196,7 +199,11 @@ class RaggedBatch:
                 lo = begin[tile] + part * each[tile]
                 hi = np.minimum(lo + each[tile], (begin + steps)[tile])
                 slot = np.where(cut[tile], first[tile] + part, -1)
-                parts += [np.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1).ravel(), np.stack([t0, t1, first, count], 1)[cut].ravel()]
+                order = np.argsort(lo - hi, kind="stable")  # long parts first
+                if len(order) * each_part <= most:  # all at once: a CU's next part is as short as its first one is long
+                    turn = max(1, _CUS // each_part)
+                    order = np.concatenate([order[i: i + turn][:: -1 if i // turn % 2 else 1] for i in range(0, len(order), turn)])
+                parts += [np.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1)[order].ravel(), np.stack([t0, t1, first, count], 1)[cut].ravel()]
                 sizes += [len(tile), int(cut.sum()), int(slots.sum())]
             self._rows[key] = to_device(np.concatenate(parts).tolist(), torch.int32, self.cu.device, self.ordered), sizes
         return self._rows[key]

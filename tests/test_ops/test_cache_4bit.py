@@ -428,6 +428,7 @@ def test_plan(counts, starts, group, window):
             taken = sorted(s for v in mine.values() for *_, s in v if s >= 0)
             assert taken == list(range(used))
             for (_, seq, t0, t1), v in mine.items():
+                v.sort()
                 first = batch.start_host[seq] + t0 - batch.cu_host[seq]
                 last = first + t1 - t0 - 1
                 assert v[0][0] == (max(0, first - window + 1) // 32 if window else 0) and v[-1][1] == last // 32 + 1
