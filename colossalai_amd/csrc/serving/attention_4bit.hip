@@ -15,6 +15,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
+#include <cmath>
 
 namespace cai {
 namespace serving {
@@ -31,7 +32,8 @@ struct Attend {
   bf16s* out;
   float* parts;
   int width, H, G, head_bytes, page_shift, window, group, subs;
-  float scale;
+  float scale;      // of the scores in base 2: positive
+  bool negative;    // so that the queries take the sign
 };
 
 // A step's codes and scales as they come.
@@ -105,7 +107,10 @@ struct Rows {
       pos[rt] = real ? a.positions[tok[rt]] : p_last;
       const bf16s* from = a.q + (real ? tok[rt] : t0) * a.q_stride + (long)(real ? head[rt] : g * a.group) * D + kg * (D / 4);
 #pragma unroll
-      for (int f = 0; f < KF; ++f) q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
+      for (int f = 0; f < KF; ++f) {
+        q[rt][f] = *reinterpret_cast<const bf16x8_v*>(from + f * 8);
+        if (a.negative) q[rt][f] = __builtin_bit_cast(bf16x8_v, __builtin_bit_cast(uint4v, q[rt][f]) ^ 0x80008000u);
+      }
       state[rt] = float2v{-INFINITY, 0.0f};
 #pragma unroll
       for (int f = 0; f < VF; ++f) o[rt][f] = f32x4{0, 0, 0, 0};
@@ -114,9 +119,9 @@ struct Rows {
 
   DEV_INLINE bool sees(const Attend& a, int rt, int key) const { return key <= pos[rt] && (a.window <= 0 || pos[rt] - key < a.window); }
 
-  // weights of the scores (base 2) of S steps as the product's operands, and with REST what bfloat16 leaves of them
-  template <bool REST, int S>
-  DEV_INLINE void weigh(const f32x4 (&s)[RT][2 * S], bf16x8_v (&p)[RT][S], bf16x8_v (&rest)[RT][S]) {
+  // A new reference where scores times `scale` (positive; base 2) of S steps would pass the old one by too much.
+  template <int S>
+  DEV_INLINE void refer(const f32x4 (&s)[RT][2 * S], float scale) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float top = -INFINITY;
@@ -125,30 +130,32 @@ struct Rows {
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
       top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32));
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
       if (__any(top > state[rt][0] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
         const float m = state[rt][0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
         state[rt] = float2v{next, state[rt][1] * fall};
 #pragma unroll
         for (int f = 0; f < VF; ++f) o[rt][f] *= fall;
       }
-      const float ref = state[rt][0] == -INFINITY ? 0.0f : state[rt][0];
+    }
+  }
+
+  // Weights of row rt's scores of a step as the product's operand, and with REST what bfloat16 leaves of them.
+  template <bool REST>
+  DEV_INLINE void weigh(int rt, const f32x4& s0, const f32x4& s1, float scale, bf16x8_v& p, bf16x8_v& rest) {
+    const float ref = state[rt][0] == -INFINITY ? 0.0f : state[rt][0];
+    float e[8];
 #pragma unroll
-      for (int step = 0; step < S; ++step) {
-        float e[8];
+    for (int i = 0; i < 8; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(i < 4 ? s0[i & 3] : s1[i & 3], scale, -ref));
+      state[rt][1] += e[i];
+    }
+    const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
+    p = __builtin_bit_cast(bf16x8_v, w);
+    if constexpr (REST) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(s[rt][2 * step + i / 4][i % 4] - ref);
-          state[rt][1] += e[i];
-        }
-        const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
-        p[rt][step] = __builtin_bit_cast(bf16x8_v, w);
-        if constexpr (REST) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-          rest[rt][step] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
-        }
-      }
+      for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      rest = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
     }
   }
 
@@ -274,7 +281,7 @@ DEV_INLINE unsigned int value_scales(const Attend& a, const Raw<D>& w, float (&s
 
 // Few rows: a block has a tile of 16 RT rows and its waves take its steps in turn.
 template <int D, int RT>
-__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2) void attention_4bit_kernel(Attend a) {
+__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2) void attention_4bit_kernel(Attend a) {
   constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;
   __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
   float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
@@ -286,7 +293,6 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   Rows<D, RT> rows;
   rows.start(a, R, 0, g, sub, t0, t1, p1, n, kg);
   const Source<D> source = {a.tables + (long)seq * a.width, p1, g};
-  const float scale = a.scale * LOG2E4;
 
   auto compute = [&](const Raw<D>& w, int step) {
     const int j = step * STEP;
@@ -304,10 +310,6 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
         for (int rt = 0; rt < RT; ++rt) s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, rows.q[rt][f], s[rt][h], 0, 0, 0);
       }
     }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[rt][h] *= scale;
     float su[2][4];
     const unsigned int odd = value_scales(a, w, su, step, p0, p1, kg, edge);
     if (edge) {
@@ -319,19 +321,21 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
           for (int i = 0; i < 4; ++i)
             s[rt][h][i] = !rows.sees(a, rt, j + h * TILE + kg * 4 + i) ? -INFINITY : odd >> (4 * h + i) & 1 ? __builtin_nanf("") : s[rt][h][i];
     }
-    bf16x8_v p[RT][1], rest[RT][1];
-    rows.template weigh<RT == 1, 1>(s, p, rest);
+    rows.template refer<1>(s, a.scale);
+    bf16x8_v p[RT], rest[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) rows.template weigh<RT == 1>(rt, s[rt][0], s[rt][1], a.scale, p[rt], rest[rt]);
     unrolled<D / 32>([&](auto byte) {
       constexpr int B = decltype(byte)::value;
       bf16x8_v lo, hi;
       value_frags<D, B>(w, su, lo, hi);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt][0], rows.o[rt][2 * B], 0, 0, 0);
-        rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt][0], rows.o[rt][2 * B + 1], 0, 0, 0);
+        rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt], rows.o[rt][2 * B], 0, 0, 0);
+        rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt], rows.o[rt][2 * B + 1], 0, 0, 0);
         if constexpr (RT == 1) {
-          rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt][0], rows.o[rt][2 * B], 0, 0, 0);
-          rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt][0], rows.o[rt][2 * B + 1], 0, 0, 0);
+          rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt], rows.o[rt][2 * B], 0, 0, 0);
+          rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt], rows.o[rt][2 * B + 1], 0, 0, 0);
         }
       }
     });
@@ -405,54 +409,61 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   else rows.store_part(a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L)), R, 0, n, kg);
 }
 
-// Many rows: a block has a tile of 32 WAVES4 rows, 32 a wave, and all its waves take the same steps. Each makes one of WAVES4 steps' codes into
-// fragments in LDS, which the others read: the conversions, half of what a wave of the other form issues, are then done once for the block.
+// Many rows: a block has 32 a wave (16 at 256 channels, where registers are few), and all its waves take the same steps. They make four steps' (two)
+// codes into fragments in LDS, each its share, which all of them read: the conversions, half of what a wave of the other form issues, are
+// then done once for the block. Two steps' scores are weighed together: the chain from scores to products is what a wave waits for (one at
+// a time: portions of 1000 over 4000 tokens 276 us, two 233; with the next step's scores formed ahead of the weights 270).
+template <int D> constexpr int shared_rows = D == 256 ? 16 : 32;   // of a wave
 template <int D>
 __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(Attend a) {
-  constexpr int RT = 2, R = 16 * RT * WAVES4, KF = D / 32, VF = D / 16;
-  __shared__ uint4v frags[WAVES4][2 * KF + VF][64];
-  __shared__ unsigned int odds[WAVES4][4];
+  constexpr int RT = shared_rows<D> / 16, R = 16 * RT * WAVES4, KF = D / 32, VF = D / 16;
+  constexpr int READY = D == 256 ? 2 : 4, SHARES = WAVES4 / READY;   // steps in LDS, waves that make one
+  __shared__ uint4v frags[READY][2 * KF + VF][64];
+  __shared__ unsigned int odds[READY][4];
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
   const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
   const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
   const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
   const int p0 = a.positions[t0], p1 = a.positions[t1 - 1], per_token = min(a.group, R), row0 = wid * 16 * RT;
+  const int made = wid / SHARES, mine = wid % SHARES;   // the step and the share of it that the wave makes
   Rows<D, RT> rows;
   rows.start(a, R, row0, g, sub, t0, t1, p1, n, kg);
-  // of the wave's own rows; without any it just works for the others
+  // of the wave's own rows; without any it works for the others
   const int mine0 = p0 + row0 / per_token, mine1 = min(p1, p0 + (row0 + 16 * RT - 1) / per_token);
   const Source<D> source = {a.tables + (long)seq * a.width, p1, g};
-  const float scale = a.scale * LOG2E4;
   Raw<D> w;
   int pages[2];
-  source.look(a, pages, from + wid);
-  source.load(a, w, from + wid, pages, n, kg);
-  for (int base = from; base < to; base += WAVES4) {
+  source.look(a, pages, from + made);
+  source.load(a, w, from + made, pages, n, kg);
+  for (int base = from; base < to; base += READY) {
     __syncthreads();   // the fragments before have been used
-    if (base + wid < to) {
-      const int step = base + wid, j = step * STEP;
+    if (base + made < to) {
+      const int step = base + made, j = step * STEP;
       const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        if (SHARES == 2 && h != mine) continue;
 #pragma unroll
-        for (int f = 0; f < KF; ++f) frags[wid][h * KF + f][lane] = __builtin_bit_cast(uint4v, key_frag(w, h, f));
+        for (int f = 0; f < KF; ++f) frags[made][h * KF + f][lane] = __builtin_bit_cast(uint4v, key_frag(w, h, f));
+      }
       float su[2][4];
       const unsigned int odd = value_scales(a, w, su, step, p0, p1, kg, edge);
-      if (n == 0) odds[wid][kg] = odd;
+      if (n == 0) odds[made][kg] = odd;
       unrolled<D / 32>([&](auto byte) {
         constexpr int B = decltype(byte)::value;
+        if (SHARES == 2 && B / (D / 64) != mine) return;
         bf16x8_v lo, hi;
         value_frags<D, B>(w, su, lo, hi);
-        frags[wid][2 * KF + 2 * B][lane] = __builtin_bit_cast(uint4v, lo);
-        frags[wid][2 * KF + 2 * B + 1][lane] = __builtin_bit_cast(uint4v, hi);
+        frags[made][2 * KF + 2 * B][lane] = __builtin_bit_cast(uint4v, lo);
+        frags[made][2 * KF + 2 * B + 1][lane] = __builtin_bit_cast(uint4v, hi);
       });
-      if (step + WAVES4 < to) {
-        source.look(a, pages, step + WAVES4);
-        source.load(a, w, step + WAVES4, pages, n, kg);
+      if (step + READY < to) {
+        source.look(a, pages, step + READY);
+        source.load(a, w, step + READY, pages, n, kg);
       }
     }
     __syncthreads();
-    const int ready = min(WAVES4, to - base);
+    const int ready = min(READY, to - base);
     // S of the steps that lie ready, from the i-th on
     auto compute = [&](auto steps, int i) {
       constexpr int S = decltype(steps)::value;
@@ -473,10 +484,6 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
       unsigned int odd = 0;
 #pragma unroll
       for (int h = 0; h < S; ++h) odd |= odds[i + h][kg] << (8 * h);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int h = 0; h < 2 * S; ++h) s[rt][h] *= scale;
       if (end > mine0 || (a.window > 0 && mine1 - j >= a.window) || __any(odd != 0)) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -486,8 +493,12 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
             for (int e = 0; e < 4; ++e)
               s[rt][h][e] = !rows.sees(a, rt, j + h * TILE + kg * 4 + e) ? -INFINITY : odd >> (4 * h + e) & 1 ? __builtin_nanf("") : s[rt][h][e];
       }
-      bf16x8_v p[RT][S], rest[RT][S];
-      rows.template weigh<false, S>(s, p, rest);
+      rows.template refer<S>(s, a.scale);
+      bf16x8_v p[RT][S], rest;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int h = 0; h < S; ++h) rows.template weigh<false>(rt, s[rt][2 * h], s[rt][2 * h + 1], a.scale, p[rt][h], rest);
 #pragma unroll
       for (int h = 0; h < S; ++h)
 #pragma unroll
@@ -580,7 +591,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void attention_4bit_join_kernel(At
   store8(a.out + ((long)tok * a.H + g * a.group + in) * D + c, o);
 }
 
-// R: rows of a tile, 16 or 32 for one wave's, 32 WAVES4 for the waves of a block
+// R: rows of a tile, 16 or 32 for one wave's, else the block's
 template <int D, int R>
 void launch(Attend a, long items, long slots, long joins, const at::Tensor& like) {
   a.subs = (a.group + R - 1) / R;
@@ -591,7 +602,7 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
     a.parts = parts.data_ptr<float>();
   }
   const dim3 grid((unsigned)(items * heads)), block(64 * WAVES4);
-  if constexpr (R == 32 * WAVES4) hipLaunchKernelGGL((attention_4bit_shared_kernel<D>), grid, block, 0, stream(), a);
+  if constexpr (R > 32) hipLaunchKernelGGL((attention_4bit_shared_kernel<D>), grid, block, 0, stream(), a);
   else hipLaunchKernelGGL((attention_4bit_kernel<D, R / 16>), grid, block, 0, stream(), a);
   HIP_CHECK_LAST();
   if (joins > 0) {
@@ -602,7 +613,7 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
 
 }  // namespace
 
-// `plan`: of the tiles with at most 16 rows, then of those with at most 32, then of those with at most 128 (heads of up to 128 channels), what a block does, (sequence, first token, end token, first step,
+// `plan`: of the tiles with at most 16 rows, then of those with at most 32, then of those with at most 128 (heads of 256 channels: 16, 64), what a block does, (sequence, first token, end token, first step,
 // end step, part or -1) for each, then the tiles that have parts, (first token, end token, first part, parts). `sizes`: of each kind the numbers of
 // both, and of parts.
 at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions,
@@ -644,7 +655,9 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   a.page_shift = 0;
   while ((1L << a.page_shift) < page_size) ++a.page_shift;
   a.window = (int)std::min<int64_t>(window, 1L << 30);
-  a.scale = (float)scale;
+  // with a scale of 0 every key has the same weight: the product with a hidden one's -infinity is to stay it
+  a.scale = std::max(std::fabs((float)scale) * LOG2E4, 1e-30f);
+  a.negative = scale < 0;
   auto run = [&](auto size) {
     constexpr int DD = decltype(size)::value;
     const int* at = plan.data_ptr<int>();
@@ -655,9 +668,8 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
       at = a.joins + 4 * joins;
       if (items == 0) continue;
       if (kind == 0) launch<DD, 16>(a, items, slots, joins, q);
-      else if (kind == 1) launch<DD, 32>(a, items, slots, joins, q);
-      else if constexpr (DD <= 128) launch<DD, 32 * WAVES4>(a, items, slots, joins, q);
-      else TORCH_CHECK_VALUE(false, who, "tiles of 128 rows are for heads of up to 128 channels");
+      else if (kind == 1) launch<DD, DD == 256 ? 16 : 32>(a, items, slots, joins, q);
+      else launch<DD, shared_rows<DD> * WAVES4>(a, items, slots, joins, q);
     }
   };
   if (D == 64) run(std::integral_constant<int, 64>());

@@ -28,7 +28,8 @@ __all__ = ["kv4_pool", "kv4_read", "kv4_unpack", "paged_kv_append", "paged_kv_ap
 
 HEAD_DIMS = (64, 128, 256)
 _NUMBERS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-_BLOCKS = {64: (1024, 768, 768), 128: (768, 512, 512), 256: (512, 256, 0)}
+# rows of the kernel's tiles by head size, and the blocks that 256 CUs hold at once, by its registers
+_TILES = {64: ((16, 32, 128), (1024, 768, 768)), 128: ((16, 32, 128), (768, 512, 512)), 256: ((16, 16, 64), (512, 512, 512))}
 _BORDERS = (0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0)
 
 
@@ -220,8 +221,7 @@ def paged_attention_4bit(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tens
     if batch.block_tables is None or window < 0:
         raise ValueError("a batch with page tables, and a window of 0 or more")
     if use_hip(q):
-        # the blocks that 256 CUs hold at once, by the kernel's registers
-        plan, sizes = batch.row_plan(H // G, G, window, _BLOCKS[D])
+        plan, sizes = batch.row_plan(H // G, G, window, *_TILES[D])
         return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.positions, plan, sizes, scale, window, batch.page_size)
     ps = _page_size(kpool, D)
     if vpool.shape != kpool.shape or vpool.dtype != torch.uint8 or batch.page_size != ps:

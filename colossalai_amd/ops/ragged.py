@@ -153,33 +153,33 @@ class RaggedBatch:
             self._even[window, fewest] = (total / (tiles * most), int(most)) if tiles else (0.5, 0)
         return self._even[window, fewest]
 
-    def row_plan(self, group: int, heads: int, window: int = 0, blocks: Sequence[int] = (1024, 512, 512), step: int = 32, least: int = 8):
+    def row_plan(self, group: int, heads: int, window: int = 0, rows: Sequence[int] = (16, 32, 128), blocks: Sequence[int] = (1024, 512, 512),
+                 step: int = 32, least: int = 8):
         """The work of an attention kernel whose block takes a tile of rows (the `group` query heads of a key head for some tokens) and a part of
-        their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles have 16
-        rows where a sequence's new tokens are at most as many rows, or one token (32 beside other tiles of 32, if they do not fill half the chip),
-        128 where they are 96 and more, else 32. A tile's keys are cut
-        into even parts of at least `least` steps, as many as the `blocks` that a chip holds at once (of tiles of 16, 32 and 128 rows; 0: no
-        such tiles) allow; `heads` key heads have a block each for a part. Longer parts come first. Built once per step
-        and kind, shared by its layers."""
+        their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles are of
+        three kinds: of the most `rows` where a sequence's new tokens fill three quarters of one, of the fewest where they fit it or are one token
+        (but not beside the second kind if they do not fill half the chip), else of the second. A tile's keys are cut into even parts of at least
+        `least` steps, as many as the `blocks` of a kind that a chip holds at once allow; `heads` key heads have a block each for a part.
+        Longer parts come first. Built once per step and kind, shared by its layers."""
         if self._rows is None:
             self._rows = {}
-        key = group, heads, window, tuple(blocks)
+        key = group, heads, window, tuple(rows), tuple(blocks)
         if key not in self._rows:
             cu, start = np.array(self.cu_host), np.array(self.start_host)
             new = cu[1:] - cu[:-1]
-            few = (new == 1) | (new * group <= 16)
-            many = ~few & (new * group >= 96) & (blocks[2] > 0)
+            few = (new == 1) | (new * group <= rows[0])
+            many = ~few & (4 * new * group >= 3 * rows[2])
             if few.sum() * heads < blocks[0] // 2 and (~few & ~many).any():  # one launch: there is room beside the others
                 few[:] = False
                 many &= new > 1
             parts, sizes = [], []
-            for rows, pick, most in ((16, few, blocks[0]), (32, ~few & ~many, blocks[1]), (128, many, blocks[2])):
+            for size, pick, most in zip(rows, (few, ~few & ~many, many), blocks):
                 seqs = np.flatnonzero(pick)
                 if not len(seqs):
                     sizes += [0, 0, 0]
                     continue
-                per = max(1, rows // group)
-                each_part = heads * -(-group // rows)  # blocks
+                per = max(1, size // group)
+                each_part = heads * -(-group // size)  # blocks
                 tiles = (new[seqs] + per - 1) // per
                 of = np.repeat(seqs, tiles)
                 t0 = cu[of] + (np.arange(len(of)) - np.repeat(tiles.cumsum() - tiles, tiles)) * per

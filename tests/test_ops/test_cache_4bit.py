@@ -411,10 +411,10 @@ def test_refusals(device):
 def test_plan(counts, starts, group, window):
     """Every key that a new token sees is in exactly one part of the token's one tile; tiles hold their rows; parts are listed with their tiles."""
     batch = RaggedBatch.build(counts, starts, list(range(len(counts))), "cpu")
-    for blocks in ((1024, 512, 512), (8, 8, 8), (1024, 512, 0)):
-        plan, sizes = batch.row_plan(group, 2, window, blocks)
+    for tiles, blocks in (((16, 32, 128), (1024, 512, 512)), ((16, 32, 128), (8, 8, 8)), ((16, 16, 64), (512, 512, 512))):
+        plan, sizes = batch.row_plan(group, 2, window, tiles, blocks)
         at, seen = 0, {}
-        for kind, rows in ((0, 16), (1, 32), (2, 128)):
+        for kind, rows in enumerate(tiles):
             items, joins, used = sizes[3 * kind: 3 * kind + 3]
             for seq, t0, t1, lo, hi, slot in plan[at: at + 6 * items].view(-1, 6).tolist():
                 assert batch.cu_host[seq] <= t0 < t1 <= batch.cu_host[seq + 1] and lo < hi
