@@ -80,6 +80,9 @@ void latent_kv_write(at::Tensor dkv, at::Tensor norm_w, double eps, at::Tensor f
 at::Tensor paged_kv_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor kpool, at::Tensor vpool, at::Tensor rows, at::Tensor positions,
                            at::Tensor table, c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, double eps);
 std::vector<at::Tensor> kv4_read(at::Tensor kpool, at::Tensor vpool, at::Tensor rows, int64_t D);
+std::tuple<at::Tensor, std::vector<int64_t>> row_plan(const std::vector<int64_t>& cu, const std::vector<int64_t>& start, int64_t group, int64_t heads,
+                                                      int64_t window, const std::vector<int64_t>& rows, const std::vector<int64_t>& blocks,
+                                                      int64_t step, int64_t least, bool pinned);
 at::Tensor paged_attention_4bit(at::Tensor q, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions, at::Tensor plan,
                                 std::vector<int64_t> sizes, double scale, int64_t window, int64_t page_size);
 std::vector<at::Tensor> expert_sort(at::Tensor ids, int64_t num_experts);
@@ -134,6 +137,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("latent_kv_write", &s::latent_kv_write, "latent row: RMS norm + pair rotation + scatter into pool rows");
   m.def("paged_kv_append", &s::paged_kv_append,
         "norm and rotation of new queries and keys; keys and values into pool rows, in their type or in 4 bits");
+  m.def("row_plan", &s::row_plan, "tiles of rows and parts of their keys of a step's attention");
   m.def("kv4_read", &s::kv4_read, "the numbers of a 4-bit cache's rows");
   m.def("paged_attention_4bit", &s::paged_attention_4bit, "ragged paged attention over a 4-bit cache");
   m.def("expert_ffn_gemv", &s::expert_ffn_gemv, "chosen experts' feed-forward of a small step, matrix-vector kernels");

@@ -12,14 +12,12 @@ else shares the step.
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
-import numpy as np
 import torch
 
 from ._kernels import serving_kernels
 
 __all__ = ["RaggedBatch", "to_device"]
 
-_CUS = 256  # of a chip
 LISTED_TOKENS = 32  # up to here a step's per-token vectors are made on the host: a launch takes as long
 
 
@@ -59,18 +57,6 @@ def to_device(values: Sequence, dtype, device, ordered: bool = False) -> torch.T
         return torch.tensor(values, dtype=dtype, pin_memory=True).to(device, non_blocking=True)
 
     return copy() if ordered else complete(copy, device)
-
-
-def _share(steps, blocks_each: int, most: int, least: int) -> int:
-    """The longest part, in steps, that tiles of ``steps`` are cut into: where their blocks (`blocks_each` a part) leave some of the `most` that a
-    chip holds at once, the smallest parts that still are all at once, `least` steps at least; else none is cut."""
-    lo, hi = least, int(steps.max())
-    if len(steps) * blocks_each >= most:
-        return hi
-    while lo < hi:
-        mid = (lo + hi) // 2
-        lo, hi = (lo, mid) if int((-(-steps // mid)).sum()) * blocks_each <= most else (mid + 1, hi)
-    return hi
 
 
 @dataclass
@@ -153,7 +139,7 @@ class RaggedBatch:
             self._even[window, fewest] = (total / (tiles * most), int(most)) if tiles else (0.5, 0)
         return self._even[window, fewest]
 
-    def row_plan(self, group: int, heads: int, window: int = 0, rows: Sequence[int] = (16, 32, 128), blocks: Sequence[int] = (1024, 512, 512),
+    def row_plan(self, group: int, heads: int, window: int = 0, rows: Sequence[int] = (16, 32, 128), blocks: Sequence[int] = (768, 512, 512),
                  step: int = 32, least: int = 8):
         """The work of an attention kernel whose block takes a tile of rows (the `group` query heads of a key head for some tokens) and a part of
         their keys, in steps of `step`: ``(plan, sizes)`` as ``paged_attention_4bit`` (csrc/serving/attention_4bit.hip) wants them. Tiles are of
@@ -165,47 +151,13 @@ class RaggedBatch:
             self._rows = {}
         key = group, heads, window, tuple(rows), tuple(blocks)
         if key not in self._rows:
-            cu, start = np.array(self.cu_host), np.array(self.start_host)
-            new = cu[1:] - cu[:-1]
-            few = (new == 1) | (new * group <= rows[0])
-            many = ~few & (4 * new * group >= 3 * rows[2])
-            if few.sum() * heads < blocks[0] // 2 and (~few & ~many).any():  # one launch: there is room beside the others
-                few[:] = False
-                many &= new > 1
-            parts, sizes = [], []
-            for size, pick, most in zip(rows, (few, ~few & ~many, many), blocks):
-                seqs = np.flatnonzero(pick)
-                if not len(seqs):
-                    sizes += [0, 0, 0]
-                    continue
-                per = max(1, size // group)
-                each_part = heads * -(-group // size)  # blocks
-                tiles = (new[seqs] + per - 1) // per
-                of = np.repeat(seqs, tiles)
-                t0 = cu[of] + (np.arange(len(of)) - np.repeat(tiles.cumsum() - tiles, tiles)) * per
-                t1 = np.minimum(t0 + per, cu[of + 1])
-                shift = start[of] - cu[of]
-                begin = np.maximum(t0 + shift - window + 1, 0) // step if window > 0 else np.zeros_like(t0)
-                steps = (t1 - 1 + shift) // step + 1 - begin
-                share = _share(steps, each_part, most, least)
-                count = -(-steps // share)
-                each = -(-steps // count)
-                count = -(-steps // each)  # none is empty
-                cut = count > 1
-                slots = count * cut
-                first = slots.cumsum() - slots
-                tile = np.repeat(np.arange(len(of)), count)
-                part = np.arange(len(tile)) - (count.cumsum() - count)[tile]
-                lo = begin[tile] + part * each[tile]
-                hi = np.minimum(lo + each[tile], (begin + steps)[tile])
-                slot = np.where(cut[tile], first[tile] + part, -1)
-                order = np.argsort(lo - hi, kind="stable")  # long parts first
-                if len(order) * each_part <= most:  # all at once: a CU's next part is as short as its first one is long
-                    turn = max(1, _CUS // each_part)
-                    order = np.concatenate([order[i: i + turn][:: -1 if i // turn % 2 else 1] for i in range(0, len(order), turn)])
-                parts += [np.stack([of[tile], t0[tile], t1[tile], lo, hi, slot], 1)[order].ravel(), np.stack([t0, t1, first, count], 1)[cut].ravel()]
-                sizes += [len(tile), int(cut.sum()), int(slots.sum())]
-            self._rows[key] = to_device(np.concatenate(parts).tolist(), torch.int32, self.cu.device, self.ordered), sizes
+            device = self.cu.device
+            if device.type == "cuda":
+                refuse_capture()
+            plan, sizes = serving_kernels().row_plan(self.cu_host, self.start_host, group, heads, window, rows, blocks, step, least,
+                                                     device.type == "cuda")
+            copy = lambda: plan.to(device, non_blocking=True)  # noqa: E731
+            self._rows[key] = complete(copy, device) if device.type == "cuda" and not self.ordered else copy(), sizes
         return self._rows[key]
 
     @property
