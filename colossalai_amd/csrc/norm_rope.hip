@@ -8,8 +8,11 @@
 //
 // Bound by memory: forward and backward read and write every value once. A wave takes a token: the lanes of a head (D / 16 of
 // them, 8 channels of each half a lane, 16-byte loads) form its sums by exchanges among themselves, 64 / lanes heads at a time,
-// and the token's angles and both weights stay in registers over all its heads. The weights' gradients are summed in registers over a
-// block's tokens, then in LDS, and the blocks' sums meet in a second launch, always in the same order.
+// and the token's angles and the weights stay in registers over all its heads. The weights' gradients are summed in registers over a
+// block's tokens, then in LDS, and the blocks' sums meet in a second launch, always in the same order. In the backward, blocks take queries
+// or keys, so that one weight and its gradient are in registers.
+// 4 x 8192 tokens, 32/8 heads of 128 in bfloat16: forward 178 us (4.5 TB/s), backward 237 (4.8; with both kinds in a block 343, without the next
+// head's values on their way 275). As elementary operations both take 7400 us.
 
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
@@ -171,15 +174,27 @@ __global__ __launch_bounds__(NR_BLOCK) void norm_rope_bwd_kernel(T* __restrict__
     T* out = dx + (token * all + first) * h.D + at;
     float c[8], s[8];
     load_angles(c, s, h, token, ss, at, half, on);
+    // the next head's values are on their way while a head is worked on, where they are two bytes (else they take a wave's room)
+    constexpr bool AHEAD = sizeof(T) == 2;
+    Eight<T> lo, hi, glo, ghi, lo2, hi2, glo2, ghi2;
+    auto load = [&](int head, Eight<T>& a, Eight<T>& b, Eight<T>& c, Eight<T>& d) {
+      if (!on || head >= heads) return;
+      a.load(row + (long)head * h.D);
+      b.load(row + (long)head * h.D + half);
+      c.load(grad + (long)head * h.D);
+      d.load(grad + (long)head * h.D + half);
+    };
+    if (AHEAD) load(side, lo2, hi2, glo2, ghi2);
 #pragma unroll 1
     for (int head = side; head < heads; head += SIDE) {
-      Eight<T> lo, hi, glo, ghi;
+      if (AHEAD) {
+        lo = lo2, hi = hi2, glo = glo2, ghi = ghi2;
+        load(head + SIDE, lo2, hi2, glo2, ghi2);
+      } else {
+        load(head, lo, hi, glo, ghi);
+      }
       float sum = 0.0f, dot = 0.0f, a[16];
       if (on) {
-        lo.load(row + (long)head * h.D);
-        hi.load(row + (long)head * h.D + half);
-        glo.load(grad + (long)head * h.D);
-        ghi.load(grad + (long)head * h.D + half);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float p = glo.get(i), r = ghi.get(i), u = lo.get(i), v = hi.get(i);
@@ -360,8 +375,11 @@ std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq_in, at::Tensor dk_in, at::Te
     TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.numel() == h.tokens * h.D * (t.is_same(dq) ? Hq : Hkv),
                 "qkv_norm_rope: gradients have the outputs' shapes and type");
   const auto dx = at::empty({x.size(0), x.size(1), x.size(2)}, x.options()), dwq = at::empty_like(wq), dwk = at::empty_like(wk);
-  // A block's sums are 2 D floats; 1024 blocks are 16 waves a CU
-  const int grid = capped_grid((h.tokens + NR_WAVES - 1) / NR_WAVES, 1024);
+  // Three tokens a wave make up for a block's weights and sums, while there are blocks for every CU. Three waves a SIMD are 768 blocks, 384 of
+  // each kind, at once: a few more would wait for all of them (5003 tokens of 20 heads of 96 in float32: 28 us with 384 and fewer, 36 with 417),
+  // many even the kinds' shares out (4 x 8192 tokens, 32/8 heads of 128: 1024 236 us, 384 of each 325)
+  const long one = (h.tokens + NR_WAVES - 1) / NR_WAVES, some = std::min<long>({one, 1024, std::max<long>(256, one / 3)});
+  const int grid = (int)(some > 384 && some < 576 ? 384 : some);
   const auto part = at::empty({(long)grid * 2 * h.D}, x.options().dtype(at::kFloat));
   auto stream = at::hip::getCurrentHIPStream();
   NR_DISPATCH(x.scalar_type(), h.D, {
