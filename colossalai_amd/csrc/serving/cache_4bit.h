@@ -44,9 +44,9 @@ DEV_INLINE float scale_of(unsigned int byte) { return __builtin_bit_cast(float, 
 // bytes of a page's head
 inline int64_t page_bytes(int64_t page_size, int64_t D) { return page_size / TILE * (TILE * D / 2 + TILE * D / 32); }
 
-// The page size of a pool of heads of D channels; 0 if it is no such pool.
+// The page size of a pool of heads of D channels; 0 if it is no such pool, or does not lie at a 16-byte address.
 inline int64_t page_size_of(const at::Tensor& pool, int64_t D) {
-  if (pool.dim() != 3 || pool.scalar_type() != at::kByte || !pool.is_contiguous()) return 0;
+  if (pool.dim() != 3 || pool.scalar_type() != at::kByte || !pool.is_contiguous() || reinterpret_cast<uintptr_t>(pool.data_ptr()) % 16 != 0) return 0;
   const int64_t ps = pool.size(2) * 32 / (17 * D);
   return ps >= TILE && (ps & (ps - 1)) == 0 && page_bytes(ps, D) == pool.size(2) ? ps : 0;
 }

@@ -270,7 +270,8 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
     TORCH_CHECK_VALUE(D == 64 || D == 128 || D == 256, who, "4-bit pools take heads of 64, 128 or 256 channels, got ", D);
     const int64_t ps = page_size_of(kpool, D);
     TORCH_CHECK_VALUE(ps > 0 && kpool.size(1) == G && vpool.sizes() == kpool.sizes() && page_size_of(vpool, D) == ps, who,
-                "4-bit pools must be contiguous uint8 [pages, ", G, ", page size * 17 * ", D, " / 32], page sizes powers of two from 16 on");
+                "4-bit pools must be contiguous uint8 [pages, ", G, ", page size * 17 * ", D, " / 32] at 16-byte addresses, page sizes powers of two from "
+                "16 on");
     a.page_shift = log2_of(ps);
     a.pool_rows = kpool.size(0) * ps;
   } else {
@@ -283,6 +284,7 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
     a.page_shift = 0;
     a.pool_rows = kpool.size(0) * kpool.size(1);
   }
+  TORCH_CHECK_VALUE(N < (1L << 31) - CA_WAVES && Hq > 0 && G > 0, who, "up to 2^31 tokens, one head at least");
   const at::Tensor out = at::empty({N, Hq, D}, q.options());
   if (N == 0) return out;
   a.tokens = N;

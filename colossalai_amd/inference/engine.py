@@ -20,6 +20,8 @@ __all__ = ["LLMEngine"]
 class LLMEngine:
     def __init__(self, model: LlamaForCausalLM, config: Optional[InferenceConfig] = None):
         self.config = config or InferenceConfig()
+        if self.config.kv_cache_bits != 16:
+            raise ValueError("4-bit caches are paged: ContinuousBatchEngine serves them")
         self.model = model.eval()
         self.device = next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype

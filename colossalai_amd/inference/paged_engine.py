@@ -81,6 +81,8 @@ class ContinuousBatchEngine:
                                  num_blocks=num_blocks, block_size=block_size,
                                  device=self.device, dtype=self.dtype, bits=self.config.kv_cache_bits)
         self.packed = self.kv.bits == 4 or getattr(attn0, "qk_norm", False)
+        if self.packed and getattr(attn0, "pir_factor", 0) != 0:
+            raise ValueError("partial interleaved rotary heads are not served over 4-bit caches or with norms")
         if self.kv.bits == 4 and torch.device(self.device).type == "cuda" and self.dtype != torch.bfloat16:
             raise ValueError(f"a 4-bit cache on a GPU serves bfloat16 models, got {self.dtype}")
         self.rm = RequestManager(self.kv, max_batch_size=self.config.max_batch_size)

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from colossalai_amd.inference import ContinuousBatchEngine, GenerationConfig, InferenceConfig, KVCacheManager
+from colossalai_amd.inference import ContinuousBatchEngine, GenerationConfig, InferenceConfig, KVCacheManager, LLMEngine
 from colossalai_amd.models import LlamaConfig, LlamaForCausalLM
 
 gpu = pytest.mark.gpu
@@ -142,6 +142,10 @@ def test_refusals():
         _engine(_model(True), 4, block_size=8)
     with pytest.raises(ValueError):
         KVCacheManager(2, 2, 64, num_blocks=4, device="cpu", layer_shapes=[(2, 64, 64)] * 2, bits=4)
+    with pytest.raises(ValueError):
+        LLMEngine(_model(False), InferenceConfig(kv_cache_bits=4))
+    with pytest.raises(ValueError):
+        _engine(_model(False, partial_interleaved_rotary_factor=0.5), 4)
     kv = KVCacheManager(1, 2, 64, num_blocks=4, device="cpu", bits=4)
     kv.allocate(0, 20)
     for call in (lambda: kv.write_prefill(0, 0, torch.zeros(3, 2, 64), torch.zeros(3, 2, 64)),

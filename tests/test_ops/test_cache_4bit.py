@@ -253,11 +253,12 @@ def _check_attention(counts, starts, H, G, D, page, window=0, device="cuda", sca
 DECODE = [
     ([1], [0], 1, 1, 64, 16), ([1], [0], 16, 2, 128, 64), ([1], [15], 4, 4, 256, 16), ([1], [16], 3, 1, 64, 32), ([1] * 3, [31, 32, 33], 7, 1, 128, 16),
     ([1] * 5, [0, 4999, 63, 1024, 2047], 8, 2, 128, 16), ([1] * 2, [9000, 3], 28, 4, 128, 64), ([1], [20011], 8, 1, 64, 16), ([1] * 4, [700, 3000, 1, 40], 20, 1, 128, 32),
-    ([1] * 3, [1500, 2, 5000], 40, 2, 256, 64), ([1] * 70, list(range(0, 1400, 20)), 4, 2, 64, 16)]
+    ([1] * 3, [1500, 2, 5000], 40, 2, 256, 64), ([1] * 2, [3000, 7], 130, 1, 64, 16), ([1] * 70, list(range(0, 1400, 20)), 4, 2, 64, 16)]
 PORTIONS = [
     ([2], [0], 4, 2, 64, 16), ([16], [0], 1, 1, 128, 16), ([17, 1, 5], [3, 100, 0], 4, 2, 128, 16), ([33, 1, 96, 65], [0, 130, 31, 64], 8, 2, 128, 16),
     ([200], [1000], 7, 1, 64, 32), ([3, 64], [5000, 10], 6, 2, 256, 64), ([300, 40], [0, 77], 20, 1, 128, 16), ([2, 2, 1], [40, 3000, 6], 40, 2, 64, 16),
-    ([513], [0], 12, 4, 256, 128), ([4, 4, 4], [10, 200, 4000], 4, 1, 128, 16)]
+    ([513], [0], 12, 4, 256, 128), ([37, 1, 2], [100, 300, 20], 70, 1, 128, 16), ([9], [500], 260, 2, 64, 32), ([5], [60], 130, 1, 256, 16),
+    ([95, 96, 24, 1], [10, 0, 2000, 50], 4, 4, 128, 16), ([40] * 9, [3000] * 9, 4, 1, 64, 64), ([4, 4, 4], [10, 200, 4000], 4, 1, 128, 16)]
 
 
 @gpu
@@ -399,6 +400,12 @@ def test_refusals(device):
         with pytest.raises(ValueError):
             paged_attention_4bit(**good | bad)
     if device == "cuda":
+        room = torch.zeros(pool.numel() + 8, dtype=torch.uint8, device=device)
+        apart = room[8:].view(pool.shape)
+        for call in (lambda: paged_attention_4bit(**good | dict(kpool=apart, vpool=apart)), lambda: kv4_read(apart, apart, rows, D),
+                     lambda: paged_kv_append(q, k, k, apart, apart, rows, rows, table)):
+            with pytest.raises(ValueError):
+                call()
         with pytest.raises(ValueError):
             paged_attention_4bit(**good | dict(q=q.float()))
         with pytest.raises(ValueError):

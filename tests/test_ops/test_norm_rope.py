@@ -177,6 +177,16 @@ def test_gradients_of_gradients_and_unused_parts():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_that_are_broadcast(dtype):
+    """Gradients of one value for all channels, heads or tokens, as sums leave them."""
+    B, S, H, G, D = 2, 21, 4, 2, 64
+    qkv, ws, grads = _inputs(B, S, H, G, D, dtype, False, "cuda")
+    spread = [grads[0][:1, :1, :1, :1].expand_as(grads[0]), grads[1][:, :, :1].expand_as(grads[1]), grads[2][:1].expand_as(grads[2])]
+    _check(qkv, ws, spread, build_rope_table(S, D, 1e4, "cuda"), H, G, None)
+
+
+@gpu
 def test_another_stream_and_a_captured_graph():
     B, S, H, G, D = 2, 64, 4, 2, 64
     table = build_rope_table(S, D, 1e4, "cuda")
