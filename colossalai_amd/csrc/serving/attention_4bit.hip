@@ -129,9 +129,9 @@ struct Rows {
       for (int h = 0; h < 2 * S; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, s[rt][h][i]);
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-      if (__any(top > state[rt][0] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
+      if (__any(top * scale > state[rt][0] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32)) * scale;
         const float m = state[rt][0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
         state[rt] = float2v{next, state[rt][1] * fall};
 #pragma unroll
@@ -409,15 +409,199 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
   else rows.store_part(a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L)), R, 0, n, kg);
 }
 
-// Many rows: a block has 32 a wave (16 at 256 channels, where registers are few), and all its waves take the same steps. They make four steps' (two)
-// codes into fragments in LDS, each its share, which all of them read: the conversions, half of what a wave of the other form issues, are
-// then done once for the block. Two steps' scores are weighed together: the chain from scores to products is what a wave waits for (one at
-// a time: portions of 1000 over 4000 tokens 276 us, two 233; with the next step's scores formed ahead of the weights 270).
-template <int D> constexpr int shared_rows = D == 256 ? 16 : 32;   // of a wave
+// Rows of a wave of the kernel below: 32, a lane and its half-wave twin have one as their column of products of 32 x 32 x 16. Of a step's 32 keys a
+// lane has those at key_of(i), in the order that the second product takes them.
+template <int D>
+struct WideRows {
+  static constexpr int KQ = D / 16, VB = D / 32;   // products of a step's scores; pairs of a lane's channels, 32 channels each
+  bf16x8_v q[KQ];
+  int pos, tok, head;
+  f32x16 o[VB];
+  float2v state;   // the reference, and the sum of the weights
+  static DEV_INLINE int key_of(int i, int hf) { return (i & 3) + 8 * (i >> 2) + 4 * hf; }
+
+  DEV_INLINE void start(const Attend& a, int R, int row0, int g, int sub, int t0, int t1, int p_last, int lane) {
+    const int per_token = min(a.group, R), hf = lane >> 5, r = row0 + (lane & 31), in = sub * R + r % per_token;
+    tok = t0 + r / per_token;
+    const bool real = tok < t1 && in < a.group;
+    head = real ? g * a.group + in : -1;
+    pos = real ? a.positions[tok] : p_last;
+    const bf16s* from = a.q + (real ? tok : t0) * a.q_stride + (long)(real ? head : g * a.group) * D;
+#pragma unroll
+    for (int j = 0; j < KQ; ++j) {   // quarter 2 (j / VB) + hf of the channels, 8 from word j % VB on
+      q[j] = *reinterpret_cast<const bf16x8_v*>(from + (2 * (j / VB) + hf) * (D / 4) + j % VB * 8);
+      if (a.negative) q[j] = __builtin_bit_cast(bf16x8_v, __builtin_bit_cast(uint4v, q[j]) ^ 0x80008000u);
+    }
+    state = float2v{-INFINITY, 0.0f};
+#pragma unroll
+    for (int b = 0; b < VB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+  }
+
+  DEV_INLINE bool sees(const Attend& a, int key) const { return key <= pos && (a.window <= 0 || pos - key < a.window); }
+
+  template <int S>
+  DEV_INLINE void refer(const f32x16 (&s)[S], float scale) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < S; ++h)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
+    if (__any(top * scale > state[0] + SLACK)) {
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale;
+      const float m = state[0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      state = float2v{next, state[1] * fall};
+#pragma unroll
+      for (int b = 0; b < VB; ++b) o[b] *= fall;
+    }
+  }
+
+  DEV_INLINE void weigh(const f32x16& s, float scale, bf16x8_v (&p)[2]) {
+    const float ref = state[0] == -INFINITY ? 0.0f : state[0];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + i], scale, -ref));
+        state[1] += e[i];
+      }
+      p[h] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
+    }
+  }
+
+  // channels of n = key_of(i), i < 8: n * (D / 16) + 2 b + (0 or 1)
+  DEV_INLINE void store(const Attend& a, int hf) const {
+    if (head < 0) return;
+    const float inv = 1.0f / state[1];
+    bf16s* to = a.out + ((long)tok * a.H + head) * D;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      unsigned int w[VB];
+#pragma unroll
+      for (int b = 0; b < VB; ++b) w[b] = two_bf16(o[b][i] * inv, o[b][i + 8] * inv);
+      unsigned int* at = reinterpret_cast<unsigned int*>(to + key_of(i, hf) * (D / 16));
+#pragma unroll
+      for (int b = 0; b < VB; b += 2) *reinterpret_cast<uint2*>(at + b) = make_uint2(w[b], w[b + 1]);
+    }
+  }
+  DEV_INLINE void store_part(float* part, int R, int r, int hf) const {
+    if (head < 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int b = 0; b < VB; b += 2)
+        *reinterpret_cast<float4v*>(part + (long)r * D + key_of(i, hf) * (D / 16) + 2 * b) = float4v{o[b][i], o[b][i + 8], o[b + 1][i], o[b + 1][i + 8]};
+    if (hf == 0) *reinterpret_cast<float2v*>(part + (long)R * D + r * 2) = state;
+  }
+};
+
+// Many rows: a block has 32 a wave, and all its waves take the same steps. Each makes one of four steps' codes into fragments in LDS, which all of them
+// read: the conversions, half of what a wave of the other form issues, are then done once for the block. Two steps' scores are weighed
+// together: the chain from scores to products is what a wave waits for. Portions of 1000 over 4000 tokens, four sequences, 32/8 heads of 128: 276 us
+// with products of 16 x 16 x 32 and a step at a time, 227 with two, 210 with products of 32 x 32 x 16, half the instructions (950 TFLOP/s).
+template <int D>
+__global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_wide_kernel(Attend a) {
+  constexpr int R = 32 * WAVES4, KF = D / 32, KQ = D / 16, VB = D / 32;
+  __shared__ uint4v keys[WAVES4][KQ][64], values[WAVES4][2][VB][64];   // of four steps
+  __shared__ unsigned int odds[WAVES4][4];
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, hf = lane >> 5;
+  const int g = (int)(blockIdx.x % a.G), sub = (int)(blockIdx.x / a.G % a.subs);
+  const int* item = a.items + (long)(blockIdx.x / a.G / a.subs) * 6;
+  const int seq = item[0], t0 = item[1], t1 = item[2], from = item[3], to = item[4], slot = item[5];
+  const int p0 = a.positions[t0], p1 = a.positions[t1 - 1], per_token = min(a.group, R), row0 = wid * 32;
+  WideRows<D> rows;
+  rows.start(a, R, row0, g, sub, t0, t1, p1, lane);
+  // of the wave's own rows; without any it works for the others
+  const int mine0 = p0 + row0 / per_token, mine1 = min(p1, p0 + (row0 + 31) / per_token);
+  const Source<D> source = {a.tables + (long)seq * a.width, p1, g};
+  Raw<D> w;
+  int pages[2];
+  source.look(a, pages, from + wid);
+  source.load(a, w, from + wid, pages, n, kg);
+  for (int base = from; base < to; base += WAVES4) {
+    __syncthreads();   // the fragments before have been used
+    if (base + wid < to) {
+      const int step = base + wid, j = step * STEP;
+      const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int f = 0; f < KF; ++f)
+          keys[wid][(kg >> 1) * KF + f][(kg & 1) * 32 + h * 16 + n] = __builtin_bit_cast(uint4v, key_frag(w, h, f));
+      float su[2][4];
+      const unsigned int odd = value_scales(a, w, su, step, p0, p1, kg, edge);
+      if (n == 0) odds[wid][kg] = odd;
+      unrolled<VB>([&](auto byte) {
+        constexpr int B = decltype(byte)::value;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          unsigned int lo[2], hi[2];
+          value_words<D, B>(w.v[h], su[h], lo, hi);
+          uint2* at = reinterpret_cast<uint2*>(&values[wid][h][B][(kg & 1) * 32 + n]) + (kg >> 1);
+          at[0] = make_uint2(lo[0], lo[1]);
+          at[32] = make_uint2(hi[0], hi[1]);   // 16 lanes on
+        }
+      });
+      if (step + WAVES4 < to) {
+        source.look(a, pages, step + WAVES4);
+        source.load(a, w, step + WAVES4, pages, n, kg);
+      }
+    }
+    __syncthreads();
+    const int ready = min(WAVES4, to - base);
+    // S of the steps that lie ready, from the first-th on
+    auto compute = [&](auto steps, int first) {
+      constexpr int S = decltype(steps)::value;
+      const int j = (base + first) * STEP, end = j + S * STEP - 1;
+      if (mine0 > mine1 || j > mine1 || (a.window > 0 && mine0 - end >= a.window)) return;   // nothing to see
+      f32x16 s[S];
+      unsigned int odd = 0;
+#pragma unroll
+      for (int h = 0; h < S; ++h) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[h][i] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < KQ; ++f)
+          s[h] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, keys[first + h][f][lane]), rows.q[f], s[h], 0, 0, 0);
+        // bits of the lane's keys: quads hf and 2 + hf of both tiles
+        const unsigned int x = odds[first + h][hf], y = odds[first + h][2 + hf];
+        odd |= ((x & 15u) | (y & 15u) << 4 | (x >> 4) << 8 | (y >> 4) << 12) << (16 * h);
+      }
+      if (end > mine0 || (a.window > 0 && mine1 - j >= a.window) || __any(odd != 0)) {
+#pragma unroll
+        for (int h = 0; h < S; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[h][i] = !rows.sees(a, j + h * STEP + rows.key_of(i, hf)) ? -INFINITY : odd >> (16 * h + i) & 1 ? __builtin_nanf("") : s[h][i];
+      }
+      rows.refer(s, a.scale);
+      bf16x8_v p[S][2];
+#pragma unroll
+      for (int h = 0; h < S; ++h) rows.weigh(s[h], a.scale, p[h]);
+#pragma unroll
+      for (int h = 0; h < S; ++h)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int b = 0; b < VB; ++b)
+            rows.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, values[first + h][t][b][lane]), p[h][t], rows.o[b], 0, 0, 0);
+    };
+    int i = 0;
+    for (; i + 2 <= ready; i += 2) compute(std::integral_constant<int, 2>(), i);
+    if (i < ready) compute(std::integral_constant<int, 1>(), i);
+  }
+  rows.state[1] += __shfl_xor(rows.state[1], 32);
+  if (slot < 0) rows.store(a, hf);
+  else rows.store_part(a.parts + (((long)slot * a.subs + sub) * a.G + g) * (R * (D + 2L)), R, row0 + (lane & 31), hf);
+}
+
+// The same at 256 channels, where registers are few: 16 rows a wave, products of 16 x 16 x 32, two steps in LDS, which two waves make each.
 template <int D>
 __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(Attend a) {
-  constexpr int RT = shared_rows<D> / 16, R = 16 * RT * WAVES4, KF = D / 32, VF = D / 16;
-  constexpr int READY = D == 256 ? 2 : 4, SHARES = WAVES4 / READY;   // steps in LDS, waves that make one
+  constexpr int RT = 1, R = 16 * RT * WAVES4, KF = D / 32, VF = D / 16;
+  constexpr int READY = 2, SHARES = WAVES4 / READY;   // steps in LDS, waves that make one
   __shared__ uint4v frags[READY][2 * KF + VF][64];
   __shared__ unsigned int odds[READY][4];
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4;
@@ -442,7 +626,7 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
       const bool edge = j + STEP - 1 > p0 || (a.window > 0 && p1 - j >= a.window) || w.bad[0] || w.bad[1];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (SHARES == 2 && h != mine) continue;
+        if (h != mine) continue;
 #pragma unroll
         for (int f = 0; f < KF; ++f) frags[made][h * KF + f][lane] = __builtin_bit_cast(uint4v, key_frag(w, h, f));
       }
@@ -451,7 +635,7 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
       if (n == 0) odds[made][kg] = odd;
       unrolled<D / 32>([&](auto byte) {
         constexpr int B = decltype(byte)::value;
-        if (SHARES == 2 && B / (D / 64) != mine) return;
+        if (B / (D / 64) != mine) return;
         bf16x8_v lo, hi;
         value_frags<D, B>(w, su, lo, hi);
         frags[made][2 * KF + 2 * B][lane] = __builtin_bit_cast(uint4v, lo);
@@ -602,7 +786,8 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
     a.parts = parts.data_ptr<float>();
   }
   const dim3 grid((unsigned)(items * heads)), block(64 * WAVES4);
-  if constexpr (R > 32) hipLaunchKernelGGL((attention_4bit_shared_kernel<D>), grid, block, 0, stream(), a);
+  if constexpr (R == 32 * WAVES4) hipLaunchKernelGGL((attention_4bit_wide_kernel<D>), grid, block, 0, stream(), a);
+  else if constexpr (R > 32) hipLaunchKernelGGL((attention_4bit_shared_kernel<D>), grid, block, 0, stream(), a);
   else hipLaunchKernelGGL((attention_4bit_kernel<D, R / 16>), grid, block, 0, stream(), a);
   HIP_CHECK_LAST();
   if (joins > 0) {
@@ -669,7 +854,7 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
       if (items == 0) continue;
       if (kind == 0) launch<DD, 16>(a, items, slots, joins, q);
       else if (kind == 1) launch<DD, DD == 256 ? 16 : 32>(a, items, slots, joins, q);
-      else launch<DD, shared_rows<DD> * WAVES4>(a, items, slots, joins, q);
+      else launch<DD, (DD == 256 ? 16 : 32) * WAVES4>(a, items, slots, joins, q);
     }
   };
   if (D == 64) run(std::integral_constant<int, 64>());
