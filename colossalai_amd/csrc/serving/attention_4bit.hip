@@ -2,14 +2,21 @@
 //
 //   p_j = exp(scale q . k_j) over the keys j that the token sees,  out = sum p_j v_j / sum p_j
 //
-// A block takes 16 RT rows, the query heads of one key head for one or several tokens, and a part of their keys; its waves take steps of 32 keys
-// in turn and meet in LDS at the end. A wave works alone, on registers: codes come in one 16-byte load a tile of 16 tokens, become
-// bfloat16 by the conversion that takes two codes and their scale, and feed
-//   S^T = K Q^T (A = 16 tokens of keys, B = 16 rows of queries: a row is a lane's column, a lane has four tokens of a tile),
-//   O^T = V^T P^T (A = 16 channels of values, B = the weights where they were born: the tokens of a lane are the same in both).
+// Rows are the query heads of one key head, for one or several tokens. A block takes a tile of rows and a part of their keys, which a plan of the
+// step lists (row_plan.cpp); waves work on steps of 32 keys. Codes come in one 16-byte load a tile of 16 tokens, become bfloat16 by the
+// conversion that takes two codes and their scale, exactly, and feed
+//   S^T = K Q^T (A = tokens of keys, B = rows of queries: a row is a lane's column, a lane has the scores of some of the step's tokens),
+//   O^T = V^T P^T (A = channels of values, B = the weights where they were born: the tokens of a lane are the same in both products).
 // One pass over the keys with a running reference and sum a row; a row's weights may pass its reference by 2^8 before sums are scaled anew.
-// Weights are rounded to bfloat16 for the product, of tiles of 16 rows in two pieces, 16 of their 24 bits; their sum is that of the float32 ones. What no row sees is taken out of the values too:
-// its scale is set to 0, so that nothing behind a sequence's end shows.
+// Weights are rounded to bfloat16 for the product, of tiles of 16 rows in two pieces, 16 of their 24 bits; their sum is that of the float32 ones.
+// What no row sees is taken out of the values too: its scale is set to 0, so that nothing behind a sequence's end shows.
+//
+// Three forms, by the rows that a sequence's new tokens make:
+//   up to 16, or 17 to 95: a wave works alone, from memory to registers, and a block's waves take its steps in turn; their states meet in
+//     LDS. Bound by memory: 16 sequences of up to 32768 tokens, 32/8 heads of 128, 66 to 75 us of parts (4.7 to 5.3 TB/s) and 5 to join
+//     them; 61 sequences, a window of 4096, 28/4 heads, 28 us (4.5 TB/s). Three waves a SIMD at 128 channels: with accumulators in registers
+//     apart, two, the first took 105 us for 96. A fixed number of parts for every sequence took 96 for 82.
+//   96 and more (at 256 channels 48): a block's waves have rows of their own and share the conversions, see there. Bound by issue.
 #include "cache_4bit.h"
 
 #include <c10/core/DeviceGuard.h>

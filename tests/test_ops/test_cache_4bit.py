@@ -412,6 +412,15 @@ def test_refusals(device):
             paged_kv_append(q, k, k, pool, pool, rows, rows, table.cpu())
 
 
+def test_plan_of_one_long_sequence_beside_many():
+    """It is cut, as the others would wait for it; sequences of one length are not."""
+    for longest, cut in ((128 * 1024, True), (1024, False)):
+        batch = RaggedBatch.build([1] * 200, [longest - 1] + [1023] * 199, list(range(200)), "cpu")
+        plan, sizes = batch.row_plan(4, 8)
+        steps = [hi - lo for *_, lo, hi, _ in plan[: 6 * sizes[0]].view(-1, 6).tolist()]
+        assert (sizes[1] > 0) == cut and max(steps) <= 2 * -(-(199 * 32 + longest // 32) * 8 // 768) and steps == sorted(steps, reverse=True)
+
+
 @pytest.mark.parametrize("counts,starts", [([1, 1], [4, 0]), ([7, 1, 33, 200, 2], [0, 900, 31, 5, 3000]), ([40], [0]), ([1], [40000])])
 @pytest.mark.parametrize("group", [1, 3, 8, 16, 20, 70])
 @pytest.mark.parametrize("window", [0, 10, 1000])
@@ -443,5 +452,5 @@ def test_plan(counts, starts, group, window):
                 if len(v) == 1:
                     assert v[0][2] == -1 and (t0, t1) not in listed
                 else:
-                    assert listed[t0, t1] == (v[0][2], len(v)) and [s for *_, s in v] == list(range(v[0][2], v[0][2] + len(v)))
+                    assert len(v) <= 64 and listed[t0, t1] == (v[0][2], len(v)) and [s for *_, s in v] == list(range(v[0][2], v[0][2] + len(v)))
         assert at == plan.numel() and sorted(t for _, _, a, b in seen for t in range(a, b)) == list(range(batch.num_tokens))
