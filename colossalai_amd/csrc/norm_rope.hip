@@ -352,6 +352,7 @@ std::vector<at::Tensor> norm_rope_fwd(at::Tensor qkv, at::Tensor wq, at::Tensor 
   TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 3, "qkv_norm_rope: qkv must be [B, S, (Hq + 2 Hkv) D]");
   const c10::DeviceGuard guard(qkv.device());
   const at::Tensor x = dense_rows(qkv);
+  for (at::Tensor* t : {&wq, &wk, &table}) *t = dense(*t);
   const Heads h = heads_of(x, wq, wk, table, positions, Hq, Hkv, eps);
   const auto q = at::empty({x.size(0), x.size(1), Hq, h.D}, x.options()), k = at::empty({x.size(0), x.size(1), Hkv, h.D}, x.options());
   const auto v = at::empty_like(k);
@@ -370,6 +371,7 @@ std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq_in, at::Tensor dk_in, at::Te
   TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 3, "qkv_norm_rope: qkv must be [B, S, (Hq + 2 Hkv) D]");
   const c10::DeviceGuard guard(qkv.device());
   const at::Tensor x = dense_rows(qkv), dq = dense(dq_in), dk = dense(dk_in), dv = dense(dv_in);
+  for (at::Tensor* t : {&wq, &wk, &table}) *t = dense(*t);
   const Heads h = heads_of(x, wq, wk, table, positions, Hq, Hkv, eps);
   for (const at::Tensor& t : {dq, dk, dv})
     TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.numel() == h.tokens * h.D * (t.is_same(dq) ? Hq : Hkv),

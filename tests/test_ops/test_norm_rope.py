@@ -105,6 +105,15 @@ def test_positions_strides_and_wide_weights(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_and_tables_at_any_address(dtype):
+    qkv, ws, grads = _inputs(2, 40, 3, 1, 64, dtype, dtype == torch.float32, "cuda")
+    table = build_rope_table(64, 64).cuda()
+    apart = lambda t: torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)  # noqa: E731
+    _check(qkv, [apart(w) for w in ws], grads, apart(table), 3, 1, None)
+
+
+@gpu
 def test_small_large_and_not_finite_rows():
     """Rows of zeros and of numbers whose squares vanish beside eps; a NaN stays in its head; positions that the table does not have."""
     B, S, H, G, D = 1, 12, 2, 1, 64
