@@ -83,6 +83,8 @@ class ContinuousBatchEngine:
         self.packed = self.kv.bits == 4 or getattr(attn0, "qk_norm", False)
         if self.packed and getattr(attn0, "pir_factor", 0) != 0:
             raise ValueError("partial interleaved rotary heads are not served over 4-bit caches or with norms")
+        if self.packed and self.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"4-bit caches and normed heads are served in bfloat16 and float32, got {self.dtype}")
         if self.kv.bits == 4 and torch.device(self.device).type == "cuda" and self.dtype != torch.bfloat16:
             raise ValueError(f"a 4-bit cache on a GPU serves bfloat16 models, got {self.dtype}")
         self.rm = RequestManager(self.kv, max_batch_size=self.config.max_batch_size)

@@ -146,6 +146,8 @@ def test_refusals():
         LLMEngine(_model(False), InferenceConfig(kv_cache_bits=4))
     with pytest.raises(ValueError):
         _engine(_model(False, partial_interleaved_rotary_factor=0.5), 4)
+    with pytest.raises(ValueError):
+        _engine(_model(True, dtype=torch.float16), 16)
     kv = KVCacheManager(1, 2, 64, num_blocks=4, device="cpu", bits=4)
     kv.allocate(0, 20)
     for call in (lambda: kv.write_prefill(0, 0, torch.zeros(3, 2, 64), torch.zeros(3, 2, 64)),
