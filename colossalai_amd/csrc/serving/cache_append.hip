@@ -248,6 +248,7 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
                     "keys and values must be as many as the queries, of one size");
   for (const at::Tensor& t : {k_in, v_in, kpool, vpool, rows, positions, table, wq.value_or(q_in), wk.value_or(q_in)})
     TORCH_CHECK_VALUE(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());
+  TORCH_CHECK_VALUE(q_in.size(0) < (1L << 32) / WAVE && q_in.size(1) > 0 && k_in.size(1) > 0, who, "up to 2^26 tokens, one head at least");   // a launch's threads
   const c10::DeviceGuard guard(q_in.device());
   const at::Tensor q = head_rows(q_in), k = head_rows(k_in), v = head_rows(v_in);
   const int64_t N = q.size(0), Hq = q.size(1), D = q.size(2), G = k.size(1);
@@ -284,7 +285,6 @@ at::Tensor paged_kv_append(at::Tensor q_in, at::Tensor k_in, at::Tensor v_in, at
     a.page_shift = 0;
     a.pool_rows = kpool.size(0) * kpool.size(1);
   }
-  TORCH_CHECK_VALUE(N < (1L << 31) - CA_WAVES && Hq > 0 && G > 0, who, "up to 2^31 tokens, one head at least");
   const at::Tensor out = at::empty({N, Hq, D}, q.options());
   if (N == 0) return out;
   a.tokens = N;

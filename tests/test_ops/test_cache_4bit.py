@@ -399,7 +399,15 @@ def test_refusals(device):
                 dict(batch=RaggedBatch.build([3], [0], [0], device))):
         with pytest.raises(ValueError):
             paged_attention_4bit(**good | bad)
+    few = RaggedBatch.build([1, 2], [0, 0], [0, 1], device, [[1], [2]], 16)
+    few.block_tables = few.block_tables[:1]
+    with pytest.raises(ValueError):
+        paged_attention_4bit(**good | dict(batch=few))
     if device == "cuda":
+        many = torch.zeros(1, device=device).int().expand(1 << 26)   # tokens of a launch's threads
+        heads = q[:1, :1].expand(1 << 26, 1, D)
+        with pytest.raises(ValueError):
+            paged_kv_append(heads, heads, heads, one, one, many, many, table)
         room = torch.zeros(pool.numel() + 8, dtype=torch.uint8, device=device)
         apart = room[8:].view(pool.shape)
         for call in (lambda: paged_attention_4bit(**good | dict(kpool=apart, vpool=apart)), lambda: kv4_read(apart, apart, rows, D),
