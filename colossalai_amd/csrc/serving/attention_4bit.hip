@@ -807,7 +807,7 @@ void launch(Attend a, long items, long slots, long joins, const at::Tensor& like
 
 // `plan`: of the tiles with at most 16 rows, then of those with at most 32, then of those with at most 128 (heads of 256 channels: 16, 64), what a block does, (sequence, first token, end token, first step,
 // end step, part or -1) for each, then the tiles that have parts, (first token, end token, first part, parts). `sizes`: of each kind the numbers of
-// both, and of parts; then the number of sequences.
+// both, and of parts; then the number of sequences, and the longest's tokens.
 at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vpool, at::Tensor block_tables, at::Tensor positions,
                                 at::Tensor plan, std::vector<int64_t> sizes, double scale, int64_t window, int64_t page_size) {
   const char* who = "paged_attention_4bit: ";
@@ -822,7 +822,7 @@ at::Tensor paged_attention_4bit(at::Tensor q_in, at::Tensor kpool, at::Tensor vp
   check_i32(block_tables, "block_tables");
   check_i32(plan, "plan");
   check_i32(positions, "positions");
-  TORCH_CHECK_VALUE(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 10 && block_tables.size(0) >= sizes[9] &&
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && positions.numel() == N && sizes.size() == 11 && block_tables.size(0) >= sizes[9] && block_tables.size(1) * page_size >= sizes[10] &&
               plan.numel() == 6 * (sizes[0] + sizes[3] + sizes[6]) + 4 * (sizes[1] + sizes[4] + sizes[7]), who, "batch of other tokens");
   for (const at::Tensor& t : {kpool, vpool, block_tables, positions, plan})
     TORCH_CHECK_VALUE(t.device() == q_in.device(), who, "tensors on ", q_in.device(), " and ", t.device());

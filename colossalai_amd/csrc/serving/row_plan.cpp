@@ -99,7 +99,10 @@ std::tuple<at::Tensor, std::vector<int64_t>> row_plan(const std::vector<int64_t>
     plan.insert(plan.end(), joins.begin(), joins.end());
     for (int64_t v : {n, (int64_t)joins.size() / 4, slots}) sizes.push_back(v);
   }
+  int64_t longest = 0;
+  for (int64_t i = 0; i < B; ++i) longest = std::max(longest, start[i] + cu[i + 1] - cu[i]);
   sizes.push_back(B);
+  sizes.push_back(longest);
   const at::Tensor out = at::empty({(int64_t)plan.size()}, at::TensorOptions().dtype(at::kInt).pinned_memory(pinned));
   std::copy(plan.begin(), plan.end(), out.data_ptr<int>());
   return {out, sizes};

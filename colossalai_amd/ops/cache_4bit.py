@@ -225,6 +225,8 @@ def paged_attention_4bit(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tens
         plan, sizes = batch.row_plan(H // G, G, window, *_TILES[D])
         return serving_kernels().paged_attention_4bit(q, kpool, vpool, batch.block_tables, batch.positions, plan, sizes, scale, window, batch.page_size)
     ps = _page_size(kpool, D)
-    if vpool.shape != kpool.shape or vpool.dtype != torch.uint8 or batch.page_size != ps or batch.block_tables.shape[0] < batch.num_seqs:
-        raise ValueError(f"a table row a sequence, and both pools have one shape and the batch's pages of {batch.page_size} tokens, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
+    tables = batch.block_tables.shape
+    if (vpool.shape != kpool.shape or vpool.dtype != torch.uint8 or batch.page_size != ps or tables[0] < batch.num_seqs
+            or tables[1] * ps < batch.max_total):
+        raise ValueError(f"a table row of all its pages a sequence, and both pools have one shape and the batch's pages of {batch.page_size} tokens, got {tuple(kpool.shape)} and {tuple(vpool.shape)}")
     return paged_attention_4bit_ref(q, kpool, vpool, batch, scale, window)

@@ -400,9 +400,11 @@ def test_refusals(device):
         with pytest.raises(ValueError):
             paged_attention_4bit(**good | bad)
     few = RaggedBatch.build([1, 2], [0, 0], [0, 1], device, [[1], [2]], 16)
-    few.block_tables = few.block_tables[:1]
-    with pytest.raises(ValueError):
-        paged_attention_4bit(**good | dict(batch=few))
+    short = RaggedBatch.build([3], [15], [0], device, [[1, 2]], 16)
+    few.block_tables, short.block_tables = few.block_tables[:1], short.block_tables[:, :1].contiguous()
+    for bad in (few, short):
+        with pytest.raises(ValueError):
+            paged_attention_4bit(**good | dict(batch=bad))
     if device == "cuda":
         many = torch.zeros(1, device=device).int().expand(1 << 26)   # tokens of a launch's threads
         heads = q[:1, :1].expand(1 << 26, 1, D)
