@@ -4,6 +4,8 @@
 // a transform, a mode or a tracer wants to see goes to the Python functions (the result is empty here).
 #include <torch/extension.h>
 
+#include <limits>
+
 #include "plain.h"
 
 namespace cai {
@@ -152,13 +154,19 @@ struct FusedRopeAttention : torch::autograd::Function<FusedRopeAttention> {
   }
 };
 
-// y of norm_rope.hip in operations that autograd knows
+// y of norm_rope.hip in operations that autograd knows. As there, a position that the table does not have gives NaN: it is looked up in a row
+// of NaN behind the table's.
 at::Tensor norm_rope_known(const at::Tensor& x, const at::Tensor& w, const at::Tensor& table, const Maybe& positions, double eps) {
   const int64_t half = x.size(3) / 2;
   const at::Tensor f = x.to(at::kFloat);
   const at::Tensor y = f * at::rsqrt(f.square().mean(-1, true) + eps) * w.to(at::kFloat);
-  const at::Tensor rows = positions ? table.index_select(0, positions->reshape(-1)).view({x.size(0), x.size(1), 1, -1})
-                                    : table.slice(0, 0, x.size(1)).view({1, x.size(1), 1, -1});
+  at::Tensor rows = table.slice(0, 0, x.size(1));
+  if (positions) {
+    const at::Tensor p = positions->reshape(-1), has = p.ge(0).logical_and(p.lt(table.size(0)));
+    const at::Tensor more = at::full({1, table.size(1)}, std::numeric_limits<double>::quiet_NaN(), table.options());
+    rows = at::cat({table, more}).index_select(0, p.masked_fill(has.logical_not(), table.size(0)));
+  }
+  rows = rows.view({positions ? x.size(0) : 1, x.size(1), 1, x.size(3)});
   const at::Tensor c = rows.narrow(3, 0, half), s = rows.narrow(3, half, half), lo = y.narrow(3, 0, half), hi = y.narrow(3, half, half);
   return at::cat({lo * c - hi * s, hi * c + lo * s}, -1).to(x.scalar_type());
 }

@@ -26,6 +26,8 @@ def norm_rope_ref(x: torch.Tensor, weight: Optional[torch.Tensor], table: torch.
     if weight is not None:
         y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * weight.to(dtype)
     here = (positions >= 0) & (positions < table.shape[0])
+    if table.shape[0] == 0:
+        table = table.new_zeros(1, table.shape[1])
     rows = table.to(dtype)[torch.where(here, positions, 0).long()].masked_fill(~here.unsqueeze(-1), float("nan"))
     cos, sin = rows.unsqueeze(-2).chunk(2, -1)
     lo, hi = y.chunk(2, -1)

@@ -185,6 +185,67 @@ def test_gradients_of_gradients_and_unused_parts():
     torch.autograd.grad(plain, leaves[0], grads)
 
 
+EACH = ["cpu", pytest.param("cuda", marks=gpu)]
+
+
+def _derivatives(of, leaves, grads, by):
+    """Gradients of ``leaves`` by ``grads``, and of their product with ``by`` the gradients of all of them."""
+    leaves, grads = ([t.detach().requires_grad_() for t in ts] for ts in (leaves, grads))
+    first = torch.autograd.grad(of(*leaves), leaves, grads, create_graph=True)
+    return first, torch.autograd.grad(sum((a * b).sum() for a, b in zip(first, by)), [*leaves, *grads])
+
+
+@pytest.mark.parametrize("device", EACH)
+@pytest.mark.parametrize("placed", [False, True])
+def test_second_derivatives(placed, device):
+    """Against those of the formula in 64 bits. A float32 number has at most D + 32 < 2^7 roundings behind it, each 2^-24 of a term that is at most
+    2^3 times the tensor's largest number (nothing cancels further in random rows of one size): 2^-14 of that."""
+    B, S, H, G, D = 2, 7, 3, 2, 64
+    g = torch.Generator().manual_seed(4)
+    leaves = [torch.randn(B, S, (H + 2 * G) * D, generator=g), *(1 + 0.3 * torch.randn(D, generator=g) for _ in range(2))]
+    by = [torch.randn(t.shape, generator=g).to(device) for t in leaves]
+    grads = [torch.randn(B, S, n, D, generator=g).to(device) for n in (H, G, G)]
+    leaves, table = [t.to(device) for t in leaves], build_rope_table(40, D, 1e4, device)
+    at = torch.randint(0, 40, (B, S), generator=g).int().to(device) if placed else None
+
+    def formula(qkv, wq, wk):
+        q, k, v = qkv.view(B, S, -1, D).split([H, G, G], 2)
+        place = torch.arange(S, device=device).expand(B, S) if at is None else at.long()
+        norm = lambda x, w: x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w  # noqa: E731
+        return [_turn(norm(q, wq), table.double(), place), _turn(norm(k, wk), table.double(), place), v]
+
+    got = _derivatives(lambda *t: qkv_norm_rope(*t, table, H, G, positions=at), leaves, grads, by)
+    want = _derivatives(formula, *([t.double() for t in ts] for ts in (leaves, grads, by)))
+    for a, b in zip([*got[0], *got[1]], [*want[0], *want[1]]):
+        assert a.dtype == torch.float32 and ((a.double() - b).abs() <= 2.0 ** -14 * b.abs().amax()).all()
+
+
+@pytest.mark.parametrize("device", EACH)
+def test_second_derivatives_at_positions_that_the_table_does_not_have(device):
+    """They are NaN for those tokens' queries and keys, and what they are for all others."""
+    B, S, H, G, D = 1, 12, 2, 1, 32
+    table = build_rope_table(S, D, 1e4, device)
+    qkv, ws, grads = _inputs(B, S, H, G, D, torch.float32, False, device)
+    by = [torch.ones_like(t) for t in (qkv, *ws)]
+    by[1].zero_(), by[2].zero_()  # the weights' gradients are sums over all tokens
+    at = torch.arange(S, device=device).int()
+    want = _derivatives(lambda *t: qkv_norm_rope(*t, table, H, G, positions=at), [qkv, *ws], grads, by)
+    lost = at.clone()
+    lost[2], lost[5], lost[9] = -1, S, 2 ** 31 - 1
+    got = _derivatives(lambda *t: qkv_norm_rope(*t, table, H, G, positions=lost), [qkv, *ws], grads, by)
+    held = torch.tensor([i not in (2, 5, 9) for i in range(S)], device=device)
+    for a, b in ((got[0][0], want[0][0]), (got[1][0], want[1][0]), (got[1][3], want[1][3])):
+        a, b = (t.reshape(S, -1, D) for t in (a, b))
+        assert torch.equal(a[held], b[held])
+    for a in (got[0][0], got[1][0]):
+        a = a.view(S, -1, D)[~held]
+        assert a[:, : H + G].isnan().all() and not a[:, H + G:].isnan().any()
+    none = qkv_norm_rope(qkv, *ws, table[:0], H, G, positions=at)  # a table of no rows has no position
+    assert none[0].isnan().all() and none[1].isnan().all() and torch.equal(none[2], qkv.view(B, S, -1, D)[:, :, H + G:])
+    first, second = _derivatives(lambda *t: qkv_norm_rope(*t, table[:0], H, G, positions=at), [qkv, *ws], grads, by)
+    assert first[0].view(S, -1, D)[:, : H + G].isnan().all() and second[0].view(S, -1, D)[:, : H + G].isnan().all()
+
+
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_gradients_that_are_broadcast(dtype):
