@@ -8,7 +8,8 @@
 //   S^T = K Q^T (A = tokens of keys, B = rows of queries: a row is a lane's column, a lane has the scores of some of the step's tokens),
 //   O^T = V^T P^T (A = channels of values, B = the weights where they were born: the tokens of a lane are the same in both products).
 // One pass over the keys with a running reference and sum a row; a row's weights may pass its reference by 2^8 before sums are scaled anew.
-// Weights are rounded to bfloat16 for the product, of tiles of 16 rows in two pieces, 16 of their 24 bits; their sum is that of the float32 ones.
+// For the product a weight is two bfloat16 pieces, 16 of its 24 bits, in every form, so that a token's result does not depend on which one it is given
+// (one piece leaves 2^-8 of each term, which shows where terms cancel: portions took 205 us for 268); their sum is that of the float32 ones.
 // What no row sees is taken out of the values too: its scale is set to 0, so that nothing behind a sequence's end shows.
 //
 // Three forms, by the rows that a sequence's new tokens make:
@@ -16,7 +17,7 @@
 //     LDS. Bound by memory: 16 sequences of up to 32768 tokens, 32/8 heads of 128, 66 to 75 us of parts (4.7 to 5.3 TB/s) and 5 to join
 //     them; 61 sequences, a window of 4096, 28/4 heads, 28 us (4.5 TB/s). Three waves a SIMD at 128 channels: with accumulators in registers
 //     apart, two, the first took 105 us for 96. A fixed number of parts for every sequence took 96 for 82.
-//   96 and more (at 256 channels 48): a block's waves have rows of their own and share the conversions, see there. Bound by issue.
+//   96 and more (at 256 channels 48): a block's waves have rows of their own and share the conversions, see there. Bound by the products.
 #include "cache_4bit.h"
 
 #include <c10/core/DeviceGuard.h>
@@ -72,6 +73,14 @@ DEV_INLINE bf16x8_v frag(unsigned int a, unsigned int b, unsigned int c, unsigne
 DEV_INLINE unsigned int two_bf16(float a, float b) {
   typedef float f2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(unsigned int, __builtin_convertvector((f2{a, b}), bf16x2));
+}
+// Eight weights as a bfloat16 each, and what that leaves of them as another: 16 of their 24 bits.
+DEV_INLINE void two_pieces(float (&e)[8], bf16x8_v& p, bf16x8_v& rest) {
+  const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
+  p = __builtin_bit_cast(bf16x8_v, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  rest = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
 }
 template <int B>
 DEV_INLINE unsigned int number_pair(const unsigned int* words, float scale) { return two_numbers<B & 3>(words[B >> 2], scale); }
@@ -147,8 +156,7 @@ struct Rows {
     }
   }
 
-  // Weights of row rt's scores of a step as the product's operand, and with REST what bfloat16 leaves of them.
-  template <bool REST>
+  // Weights of row rt's scores of a step as the product's operand, and what bfloat16 leaves of them.
   DEV_INLINE void weigh(int rt, const f32x4& s0, const f32x4& s1, float scale, bf16x8_v& p, bf16x8_v& rest) {
     const float ref = state[rt][0] == -INFINITY ? 0.0f : state[rt][0];
     float e[8];
@@ -157,13 +165,7 @@ struct Rows {
       e[i] = __builtin_amdgcn_exp2f(fmaf(i < 4 ? s0[i & 3] : s1[i & 3], scale, -ref));
       state[rt][1] += e[i];
     }
-    const uint4v w = {two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7])};
-    p = __builtin_bit_cast(bf16x8_v, w);
-    if constexpr (REST) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] -= __builtin_bit_cast(float, i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-      rest = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
-    }
+    two_pieces(e, p, rest);
   }
 
   // sums of the lanes that share a row
@@ -288,7 +290,7 @@ DEV_INLINE unsigned int value_scales(const Attend& a, const Raw<D>& w, float (&s
 
 // Few rows: a block has a tile of 16 RT rows and its waves take its steps in turn.
 template <int D, int RT>
-__global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : 2) void attention_4bit_kernel(Attend a) {
+__global__ __launch_bounds__(64 * WAVES4, D == 64 ? 5 - RT : D == 128 ? 4 - RT : 2) void attention_4bit_kernel(Attend a) {
   constexpr int R = 16 * RT, KF = D / 32, VF = D / 16;
   __shared__ float4v lds[WAVES4 / 2][RT * VF][64];   // at first the waves' states
   float2v(&states)[WAVES4][R] = reinterpret_cast<float2v(&)[WAVES4][R]>(lds);
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
     rows.template refer<1>(s, a.scale);
     bf16x8_v p[RT], rest[RT];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) rows.template weigh<RT == 1>(rt, s[rt][0], s[rt][1], a.scale, p[rt], rest[rt]);
+    for (int rt = 0; rt < RT; ++rt) rows.weigh(rt, s[rt][0], s[rt][1], a.scale, p[rt], rest[rt]);
     unrolled<D / 32>([&](auto byte) {
       constexpr int B = decltype(byte)::value;
       bf16x8_v lo, hi;
@@ -340,10 +342,8 @@ __global__ __launch_bounds__(64 * WAVES4, RT == 1 ? (D == 64 ? 4 : D == 128 ? 3 
       for (int rt = 0; rt < RT; ++rt) {
         rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, p[rt], rows.o[rt][2 * B], 0, 0, 0);
         rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, p[rt], rows.o[rt][2 * B + 1], 0, 0, 0);
-        if constexpr (RT == 1) {
-          rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt], rows.o[rt][2 * B], 0, 0, 0);
-          rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt], rows.o[rt][2 * B + 1], 0, 0, 0);
-        }
+        rows.o[rt][2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(lo, rest[rt], rows.o[rt][2 * B], 0, 0, 0);
+        rows.o[rt][2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hi, rest[rt], rows.o[rt][2 * B + 1], 0, 0, 0);
       }
     });
   };
@@ -464,7 +464,7 @@ struct WideRows {
     }
   }
 
-  DEV_INLINE void weigh(const f32x16& s, float scale, bf16x8_v (&p)[2]) {
+  DEV_INLINE void weigh(const f32x16& s, float scale, bf16x8_v (&p)[2], bf16x8_v (&rest)[2]) {
     const float ref = state[0] == -INFINITY ? 0.0f : state[0];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -474,7 +474,7 @@ struct WideRows {
         e[i] = __builtin_amdgcn_exp2f(fmaf(s[8 * h + i], scale, -ref));
         state[1] += e[i];
       }
-      p[h] = frag(two_bf16(e[0], e[1]), two_bf16(e[2], e[3]), two_bf16(e[4], e[5]), two_bf16(e[6], e[7]));
+      two_pieces(e, p[h], rest[h]);
     }
   }
 
@@ -506,8 +506,9 @@ struct WideRows {
 
 // Many rows: a block has 32 a wave, and all its waves take the same steps. Each makes one of four steps' codes into fragments in LDS, which all of them
 // read: the conversions, half of what a wave of the other form issues, are then done once for the block. Two steps' scores are weighed
-// together: the chain from scores to products is what a wave waits for. Portions of 1000 over 4000 tokens, four sequences, 32/8 heads of 128: 276 us
-// with products of 16 x 16 x 32 and a step at a time, 227 with two, 210 with products of 32 x 32 x 16, half the instructions (950 TFLOP/s).
+// together: the chain from scores to products is what a wave waits for. Portions of 1000 over 4000 tokens, four sequences, 32/8 heads of 128: with
+// weights of one piece 276 us by products of 16 x 16 x 32 and a step at a time, 227 with two, 205 by products of 32 x 32 x 16, half the instructions;
+// with both pieces 268 (744 TFLOP/s, 1116 of the three products that they are).
 template <int D>
 __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_wide_kernel(Attend a) {
   constexpr int R = 32 * WAVES4, KF = D / 32, KQ = D / 16, VB = D / 32;
@@ -584,16 +585,19 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_wide_kernel(Att
             s[h][i] = !rows.sees(a, j + h * STEP + rows.key_of(i, hf)) ? -INFINITY : odd >> (16 * h + i) & 1 ? __builtin_nanf("") : s[h][i];
       }
       rows.refer(s, a.scale);
-      bf16x8_v p[S][2];
+      bf16x8_v p[S][2], rest[S][2];
 #pragma unroll
-      for (int h = 0; h < S; ++h) rows.weigh(s[h], a.scale, p[h]);
+      for (int h = 0; h < S; ++h) rows.weigh(s[h], a.scale, p[h], rest[h]);
 #pragma unroll
       for (int h = 0; h < S; ++h)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int b = 0; b < VB; ++b)
-            rows.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_v, values[first + h][t][b][lane]), p[h][t], rows.o[b], 0, 0, 0);
+          for (int b = 0; b < VB; ++b) {
+            const bf16x8_v v = __builtin_bit_cast(bf16x8_v, values[first + h][t][b][lane]);
+            rows.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, p[h][t], rows.o[b], 0, 0, 0);
+            rows.o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, rest[h][t], rows.o[b], 0, 0, 0);
+          }
     };
     int i = 0;
     for (; i + 2 <= ready; i += 2) compute(std::integral_constant<int, 2>(), i);
@@ -685,18 +689,21 @@ __global__ __launch_bounds__(64 * WAVES4, 2) void attention_4bit_shared_kernel(A
               s[rt][h][e] = !rows.sees(a, rt, j + h * TILE + kg * 4 + e) ? -INFINITY : odd >> (4 * h + e) & 1 ? __builtin_nanf("") : s[rt][h][e];
       }
       rows.template refer<S>(s, a.scale);
-      bf16x8_v p[RT][S], rest;
+      bf16x8_v p[RT][S], rest[RT][S];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int h = 0; h < S; ++h) rows.template weigh<false>(rt, s[rt][2 * h], s[rt][2 * h + 1], a.scale, p[rt][h], rest);
+        for (int h = 0; h < S; ++h) rows.weigh(rt, s[rt][2 * h], s[rt][2 * h + 1], a.scale, p[rt][h], rest[rt][h]);
 #pragma unroll
       for (int h = 0; h < S; ++h)
 #pragma unroll
         for (int f = 0; f < VF; ++f) {
           const bf16x8_v v = __builtin_bit_cast(bf16x8_v, frags[i + h][2 * KF + f][lane]);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) rows.o[rt][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rt][h], rows.o[rt][f], 0, 0, 0);
+          for (int rt = 0; rt < RT; ++rt) {
+            rows.o[rt][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, p[rt][h], rows.o[rt][f], 0, 0, 0);
+            rows.o[rt][f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, rest[rt][h], rows.o[rt][f], 0, 0, 0);
+          }
         }
     };
     int i = 0;

@@ -210,7 +210,7 @@ def paged_attention_4bit(q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tens
     """``paged_attention`` over a 4-bit cache, which already holds the step's keys (``paged_kv_append`` runs first): q [N, H, D] in bfloat16
     (token stride free), causal, limited to a sliding ``window`` if it is not 0; query head ``h`` reads head ``h // (H / G)``. Single tokens and
     prompt portions of any lengths in one call. Returns [N, H, D] in q's type. Scores, sums and the accumulation are float32; a weight is
-    rounded to bfloat16 for its product, of single tokens in two pieces. A page number that the pools do not have gives NaN to the tokens that see
+    two bfloat16 pieces for its product, 16 bits, whatever shares the step. A page number that the pools do not have gives NaN to the tokens that see
     it. The plan of a step's work is made by the first call with a batch and kept by it, not while a graph is captured."""
     if q.dim() != 3 or q.shape[0] != batch.num_tokens:
         raise ValueError(f"q must be [{batch.num_tokens}, H, D], got {tuple(q.shape)}")
