@@ -254,9 +254,23 @@ DEV_INLINE void value_frags(const Raw<D>& w, const float (&su)[2][4], bf16x8_v& 
   hi = frag(hi0[0], hi0[1], hi1[0], hi1[1]);
 }
 
+// Whether the lane's channels of token i (0 .. 3) of a tile's values, at that scale byte, have a number that is not finite: NaN at 255; infinite from
+// 2^128 on, codes of 4 and 6 at 253 and of 2 and more at 254.
+template <int D, int I>
+DEV_INLINE bool not_finite(const unsigned int (&w)[D / 32], unsigned int byte) {
+  constexpr int S = D / 32;   // bytes of a token
+  unsigned int codes = 0;     // by their two upper bits: 4 and 6 have both, 2 and more the first
+#pragma unroll
+  for (int b = 0; b < S; b += 4) {
+    const unsigned int x = w[(I * S + b) / 4] >> (I * S % 4 * 8) & (S < 4 ? (1u << (8 * S % 32)) - 1 : ~0u);
+    codes |= byte == 253 ? x & x << 1 : x;
+  }
+  return byte == 255 || (byte >= 253 && (codes & 0x44444444u) != 0);
+}
+
 // What a step's values are to be taken at: 0 for keys that no row from position p_first to p_last sees. `odd`: of the lane's keys
-// (4 h + i) those that show NaN to the rows that see them, as their page or their value's scale is none: a weight of 0 would not hide such a
-// value, so that it is taken as 0 too and goes to the rows through their scores.
+// (4 h + i) those that show NaN to the rows that see them, as their page is none or their value has a number that is not finite: a weight of 0 would
+// not hide such a value, so that it is taken at 0 too and goes to the rows through their scores.
 template <int D>
 DEV_INLINE unsigned int value_scales(const Attend& a, const Raw<D>& w, float (&su)[2][4], int step, int p_first, int p_last, int kg, bool look) {
   unsigned int odd = 0, vs[2] = {w.vs[0], w.vs[1]};
@@ -268,17 +282,17 @@ DEV_INLINE unsigned int value_scales(const Attend& a, const Raw<D>& w, float (&s
         const int key = step * STEP + h * TILE + kg * 4 + i;
         if (key > p_last || (a.window > 0 && p_first - key >= a.window)) vs[h] &= ~(255u << (8 * i));
       }
-    auto none = [](unsigned int v) { return ((v & 0x7f7f7f7fu) + 0x01010101u) & v & 0x80808080u; };   // the bytes of 255
-    if (__any((none(vs[0]) | none(vs[1])) != 0) || w.bad[0] || w.bad[1]) {
+    auto high = [](unsigned int v) { return ((v & 0x7f7f7f7fu) + 0x03030303u) & v & 0x80808080u; };   // the bytes from 253 on
+    if (__any((high(vs[0]) | high(vs[1])) != 0) || w.bad[0] || w.bad[1]) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned long long lanes = __ballot(((vs[h] >> (8 * i)) & 255u) == 255u);
-          if (!w.bad[h] && ((lanes >> (16 * kg)) & 0xffffu) == 0) continue;
-          odd |= 1u << (4 * h + i);   // where it is not seen at all, it does not show either
-          vs[h] &= ~(255u << (8 * i));
-        }
+        unrolled<4>([&](auto token) {
+          constexpr int I = decltype(token)::value;
+          const unsigned long long lanes = __ballot(not_finite<D, I>(w.v[h], (vs[h] >> (8 * I)) & 255u));
+          if (!w.bad[h] && ((lanes >> (16 * kg)) & 0xffffu) == 0) return;
+          odd |= 1u << (4 * h + I);   // where it is not seen at all, it does not show either
+          vs[h] &= ~(255u << (8 * I));
+        });
     }
   }
 #pragma unroll

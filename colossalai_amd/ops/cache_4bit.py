@@ -200,8 +200,8 @@ def paged_attention_4bit_ref(q, kpool, vpool, batch: RaggedBatch, scale: float, 
         if window > 0:
             seen = seen & (at - key < window)
         p = torch.softmax((q[lo:hi].float().transpose(0, 1) @ kk.transpose(1, 2) * scale).masked_fill(~seen, float("-inf")), -1)
-        shown = (seen.float() @ vv.isnan().float()) > 0  # a weight of 0 hides what is not seen
-        out[lo:hi] = (p @ vv.nan_to_num(0.0)).masked_fill(shown, float("nan")).transpose(0, 1)
+        shown = (seen.float() @ (~vv.isfinite()).float()) > 0  # a weight of 0 hides what is not seen
+        out[lo:hi] = (p @ vv.nan_to_num(0.0, 0.0, 0.0)).masked_fill(shown, float("nan")).transpose(0, 1)
     return out.to(q.dtype)
 
 

@@ -68,3 +68,66 @@ def test_weights_have_16_bits(form, D):
         slack = 2.0 ** -16 + 2.0 ** -22 + 2 * (D + 2) * 2.0 ** -24 * size + 2 * keys * 2.0 ** -24
         off = (got[rows].transpose(0, 1) - want).abs() - 2.0 ** -8 * want.abs() - slack * near
         assert (off <= 0).all(), f"{float((off / near).max()):.2e} of the terms over the bound"
+
+
+def _put(pools, tables, values, seq, key, head, code, byte, group=1):
+    """One channel's code, all others of its group 0, and the group's scale byte, for a key of a sequence."""
+    pool = pools[values]
+    D = pool.shape[2] * 32 // (17 * PAGE)
+    codes, scales = _tiles(pool, D, values)
+    page, t = tables[seq][key // PAGE], key % PAGE
+    mine = codes[page, head, 0, t // 4, :, t % 4] if values else codes[page, head, 0, t]  # [16, D / 32] or [D / 2]
+    flat = mine.reshape(-1).clone()
+    flat[group * 16: group * 16 + 16] = 0
+    flat[group * 16 + 5] = code
+    mine.copy_(flat.view(mine.shape))
+    (scales[page, head, 0, :, t] if values else scales[page, head, 0, t])[group] = byte
+
+
+NOT_FINITE = [(7, 255), (0, 255), (6, 253), (15, 253), (4, 254), (13, 254)]
+FINITE = [(5, 253), (13, 253), (3, 254), (11, 254), (7, 252)]
+
+
+@sizes
+@pytest.mark.parametrize("code,byte", NOT_FINITE)
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_values_that_are_not_finite_stay_with_the_tokens_that_see_them(code, byte, device, D):
+    """NaN by the scale, infinite by the number. Tokens ahead of it, and those whose window it has left, are what they were; those that
+    see it are not finite in its channel. In steps that all tokens see, and in those that some do not."""
+    for form in FORMS:
+        batch, tables, q, clean = _step(form, D, device)
+        for window in (0, 20):
+            want = paged_attention_4bit(q, *clean, batch, D ** -0.5, window)
+            assert want.isfinite().all()
+            for seq in range(batch.num_seqs):
+                lo, hi, start = batch.cu_host[seq], batch.cu_host[seq + 1], batch.start_host[seq]
+                at = torch.arange(start, start + hi - lo, device=device)
+                for key in {0, start // 2, max(0, start - 19), start, start + (hi - lo) // 2, start + hi - lo - 1}:
+                    pools = [p.clone() for p in clean]
+                    _put(pools, tables, True, seq, key, 1, code, byte)
+                    got = paged_attention_4bit(q, *pools, batch, D ** -0.5, window)
+                    sees = torch.zeros(len(q), dtype=torch.bool, device=device)
+                    sees[lo:hi] = (key <= at) & ((at - key < window) | (window == 0))
+                    assert torch.equal(got[~sees], want[~sees]) and torch.equal(got[sees, :GROUP], want[sees, :GROUP]), (form, window, seq, key)
+                    assert not got[sees, GROUP:, 32 + 10].isfinite().any(), (form, window, seq, key)
+
+
+@sizes
+@pytest.mark.parametrize("code,byte", FINITE)
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_the_largest_values_that_are_finite(code, byte, device, D):
+    """They are no more than values: of other tokens nothing changes, and of those that see one its channel alone."""
+    batch, tables, q, clean = _step("all", D, device)
+    want = paged_attention_4bit(q, *clean, batch, D ** -0.5)
+    for seq, key in ((0, 700), (1, 0), (1, 90), (1, 131), (1, 239), (2, 304)):
+        pools, zeros = [p.clone() for p in clean], [p.clone() for p in clean]
+        _put(pools, tables, True, seq, key, 1, code, byte)
+        _put(zeros, tables, True, seq, key, 1, 0, 127)
+        got, without = (paged_attention_4bit(q, *p, batch, D ** -0.5) for p in (pools, zeros))
+        other = torch.ones(D, dtype=torch.bool, device=device)
+        other[32 + 10] = False
+        assert torch.equal(got[..., other], without[..., other])
+        sees = torch.zeros(len(q), dtype=torch.bool, device=device)
+        lo, hi = batch.cu_host[seq], batch.cu_host[seq + 1]
+        sees[lo:hi] = torch.arange(hi - lo, device=device) + batch.start_host[seq] >= key
+        assert torch.equal(got[~sees], want[~sees]) and not got[sees, GROUP:, 32 + 10].isnan().any()
