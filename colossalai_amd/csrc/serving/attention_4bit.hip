@@ -148,7 +148,8 @@ struct Rows {
       if (__any(top * scale > state[rt][0] + SLACK)) {   // -INFINITY + SLACK is -INFINITY: the first keys that a row sees come here
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-        const float m = state[rt][0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+        // a row's reference is its own affair: what the others need does not show in it
+        const float m = state[rt][0], next = top > m + SLACK ? top : m, fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
         state[rt] = float2v{next, state[rt][1] * fall};
 #pragma unroll
         for (int f = 0; f < VF; ++f) o[rt][f] *= fall;
@@ -471,7 +472,7 @@ struct WideRows {
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[h][i]);
     if (__any(top * scale > state[0] + SLACK)) {
       top = fmaxf(top, __shfl_xor(top, 32)) * scale;
-      const float m = state[0], next = fmaxf(m, top), fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
+      const float m = state[0], next = top > m + SLACK ? top : m, fall = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - next);
       state = float2v{next, state[1] * fall};
 #pragma unroll
       for (int b = 0; b < VB; ++b) o[b] *= fall;

@@ -70,6 +70,24 @@ def test_weights_have_16_bits(form, D):
         assert (off <= 0).all(), f"{float((off / near).max()):.2e} of the terms over the bound"
 
 
+@gpu
+@forms
+@sizes
+def test_a_token_is_its_own_affair(form, D):
+    """Whatever the others of its step ask for, to the last bit: their scores, up to hundreds, come at other keys."""
+    batch, tables, q, pools = _step(form, D)
+    want = paged_attention_4bit(q, *pools, batch, D ** -0.5)
+    for every in (2, 3):
+        others = torch.arange(len(q), device="cuda") % every != 0
+        again = q.clone()
+        again[others] = 40 * again[others].flip(0)
+        got = paged_attention_4bit(again, *pools, batch, D ** -0.5)
+        assert torch.equal(got[~others], want[~others])
+        again = q.clone()
+        again[:, 1::2] *= 40  # heads beside it
+        assert torch.equal(paged_attention_4bit(again, *pools, batch, D ** -0.5)[:, ::2], want[:, ::2])
+
+
 def _put(pools, tables, values, seq, key, head, code, byte, group=1):
     """One channel's code, all others of its group 0, and the group's scale byte, for a key of a sequence."""
     pool = pools[values]
