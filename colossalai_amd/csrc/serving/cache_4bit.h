@@ -38,7 +38,8 @@ template <int BYTE>
 DEV_INLINE unsigned int two_numbers(unsigned int word, float scale) {
   return __builtin_bit_cast(unsigned int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, scale, BYTE));
 }
-// 2^e of a scale's byte; 0 gives 0, 255 infinity
+// A scale's byte e + 127 as the conversion takes it: by the exponent's bits, 0 as 2^-127 (measured on gfx950), and with 255 every code, 0 too, becomes
+// NaN, so that a key of such a group makes every score NaN whatever the queries' signs (test_cache_4bit_forms.py holds the kernels to it).
 DEV_INLINE float scale_of(unsigned int byte) { return __builtin_bit_cast(float, byte << 23); }
 
 // bytes of a page's head

@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from colossalai_amd.ops import kv4_pool, paged_attention_4bit
+from colossalai_amd.ops import kv4_pool, paged_attention_4bit, paged_kv_append
 from colossalai_amd.ops.cache_4bit import _TILES, _tiles, kv4_unpack
 from colossalai_amd.ops.ragged import RaggedBatch
 
@@ -128,6 +128,46 @@ def test_values_that_are_not_finite_stay_with_the_tokens_that_see_them(code, byt
                     sees[lo:hi] = (key <= at) & ((at - key < window) | (window == 0))
                     assert torch.equal(got[~sees], want[~sees]) and torch.equal(got[sees, :GROUP], want[sees, :GROUP]), (form, window, seq, key)
                     assert not got[sees, GROUP:, 32 + 10].isfinite().any(), (form, window, seq, key)
+
+
+@sizes
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_keys_that_are_not_finite_show_whatever_the_queries_sign(sign, device, D):
+    """A group with one infinity is code 7 there and 0 elsewhere, at scale byte 255: no key that scores of minus infinity would hide."""
+    for form in FORMS:
+        batch, tables, q, clean = _step(form, D, device)
+        q = sign * q.abs()
+        want = paged_attention_4bit(q, *clean, batch, D ** -0.5)
+        for seq in range(batch.num_seqs):
+            lo, hi, start = batch.cu_host[seq], batch.cu_host[seq + 1], batch.start_host[seq]
+            for key in {0, start // 2, start, start + hi - lo - 1}:
+                for code in (7, 0):
+                    pools = [p.clone() for p in clean]
+                    _put(pools, tables, False, seq, key, 1, code, 255)
+                    got = paged_attention_4bit(q, *pools, batch, D ** -0.5)
+                    sees = torch.zeros(len(q), dtype=torch.bool, device=device)
+                    sees[lo:hi] = torch.arange(start, start + hi - lo, device=device) >= key
+                    assert torch.equal(got[~sees], want[~sees]) and torch.equal(got[sees, :GROUP], want[sees, :GROUP]), (form, seq, key)
+                    assert got[sees, GROUP:].isnan().all(), (form, seq, key)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@sizes
+def test_an_appended_infinity_shows(device, D):
+    """From the append to the attention: one infinite channel of a key, queries of one sign against it."""
+    batch = RaggedBatch.build([1], [40], [0], device, [[2, 0, 1]], PAGE)
+    pools = [kv4_pool(3, PAGE, HEADS, D, device) for _ in range(2)]
+    table = torch.cat([torch.ones(64, D // 2), torch.zeros(64, D // 2)], 1).to(device)  # turned by nothing
+    x = torch.ones(41, GROUP * HEADS + 2 * HEADS, D, device=device).bfloat16()
+    q, k, v = x.split([GROUP * HEADS, HEADS, HEADS], 1)
+    k[7, 1, 3] = math.inf
+    at = torch.arange(41, device=device).int()
+    rows = torch.tensor([2, 0, 1], device=device).int()[at // PAGE] * PAGE + at % PAGE
+    for sign in (-1, 1):
+        last = paged_kv_append(sign * q.contiguous(), k, v, *pools, rows, at, table)[-1:]
+        got = paged_attention_4bit(last, *pools, batch, D ** -0.5)
+        assert (got[:, :GROUP] == 1).all() and got[:, GROUP:].isnan().all()
 
 
 @sizes
