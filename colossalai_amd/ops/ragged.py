@@ -149,7 +149,7 @@ class RaggedBatch:
         Longer parts come first. Built once per step and kind, shared by its layers."""
         if self._rows is None:
             self._rows = {}
-        key = group, heads, window, tuple(rows), tuple(blocks)
+        key = group, heads, window, tuple(rows), tuple(blocks), step, least
         if key not in self._rows:
             device = self.cu.device
             if device.type == "cuda":

@@ -189,3 +189,13 @@ def test_the_largest_values_that_are_finite(code, byte, device, D):
         lo, hi = batch.cu_host[seq], batch.cu_host[seq + 1]
         sees[lo:hi] = torch.arange(hi - lo, device=device) + batch.start_host[seq] >= key
         assert torch.equal(got[~sees], want[~sees]) and not got[sees, GROUP:, 32 + 10].isnan().any()
+
+
+def test_plans_of_other_steps_are_others():
+    """A batch keeps a plan by all that it was asked for: steps of 16 keys are twice as many, and longer parts are fewer."""
+    batch = RaggedBatch.build([1, 1], [999, 4000], [0, 1], "cpu")
+    ends = lambda plan, sizes: plan[: 6 * sizes[0]].view(-1, 6)[:, 4].max().item()  # noqa: E731
+    first = batch.row_plan(4, 2)
+    assert ends(*first) == -(-4001 // 32) and ends(*batch.row_plan(4, 2, step=16)) == -(-4001 // 16)
+    assert batch.row_plan(4, 2, least=1000)[1][0] == 2 < first[1][0]
+    assert batch.row_plan(4, 2) is first
