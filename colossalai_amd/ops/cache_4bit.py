@@ -79,7 +79,7 @@ def _codes(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     most = x.abs().amax(-1)
     odd = ~(x.abs() <= torch.finfo(torch.float32).max).all(-1)
     mantissa, e = torch.frexp(most.masked_fill(odd, 0))
-    e = (e - 3 + (mantissa > 0.75).int()).clamp(min=-126)
+    e = (e - 3 + (mantissa > 0.75).int()).masked_fill(mantissa == 0, -126).clamp(min=-126)  # frexp calls 0 a number of 2^0
     a = torch.ldexp(x.abs(), -e.unsqueeze(-1))
     code = sum((a >= b if i % 2 else a > b).byte() for i, b in enumerate(_BORDERS))
     code = code.masked_fill(odd.unsqueeze(-1), 7) | ((x < 0).byte() << 3)

@@ -199,3 +199,21 @@ def test_plans_of_other_steps_are_others():
     assert ends(*first) == -(-4001 // 32) and ends(*batch.row_plan(4, 2, step=16)) == -(-4001 // 16)
     assert batch.row_plan(4, 2, least=1000)[1][0] == 2 < first[1][0]
     assert batch.row_plan(4, 2) is first
+
+
+@sizes
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_scale_bytes_of_zeros(device, D):
+    """The smallest power of two that clips nothing of a group of zeros is the smallest there is, byte 1; so it is for numbers up to 6 * 2^-126."""
+    pools = [kv4_pool(1, PAGE, HEADS, D, device).fill_(99) for _ in range(2)]
+    x = torch.zeros(PAGE, HEADS, D, device=device)
+    x[1], x[2], x[3] = 2.0 ** -126, 6 * 2.0 ** -126, 6.5 * 2.0 ** -126
+    at = torch.arange(PAGE, device=device).int()
+    table = torch.cat([torch.ones(PAGE, D // 2), torch.zeros(PAGE, D // 2)], 1).to(device)
+    paged_kv_append(torch.zeros(PAGE, 4, D, device=device), x, x, *pools, at, at, table)
+    for values in (False, True):
+        codes, scales = _tiles(pools[values], D, values)
+        by_token = (scales.transpose(-1, -2) if values else scales)[0, :, 0]
+        assert (by_token[:, 3] == 2).all() and (by_token[:, :3] == 1).all() and (by_token[:, 4:] == 1).all()
+        token = (lambda t: codes[0, :, 0, t // 4, :, t % 4]) if values else (lambda t: codes[0, :, 0, t])
+        assert (token(0) == 0).all() and (token(1) == 0x22).all() and (token(2) == 0x77).all()
