@@ -194,7 +194,9 @@ def paged_attention_4bit_ref(q, kpool, vpool, batch: RaggedBatch, scale: float, 
         lo, hi, s0 = batch.cu_host[i], batch.cu_host[i + 1], batch.start_host[i]
         L = s0 + hi - lo
         pages = batch.block_tables[i, : -(-L // batch.page_size)].long()
-        kk, vv = (x[pages].flatten(0, 1)[:L].repeat_interleave(H // x.shape[2], 1).transpose(0, 1) for x in (k, v))
+        here = (pages >= 0) & (pages < k.shape[0])
+        kk, vv = (x[pages * here].masked_fill(~here[:, None, None, None], float("nan")).flatten(0, 1)[:L].repeat_interleave(H // x.shape[2], 1)
+                  .transpose(0, 1) for x in (k, v))
         at, key = torch.arange(s0, L, device=q.device)[:, None], torch.arange(L, device=q.device)[None]
         seen = key <= at
         if window > 0:

@@ -171,6 +171,28 @@ def test_an_appended_infinity_shows(device, D):
 
 
 @sizes
+@pytest.mark.parametrize("page", [-1, -5, 10 ** 6])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_pages_that_the_pool_does_not_have(page, device, D):
+    """NaN to the tokens that see a key of one, and nothing to others, in every form: no page counted from the end."""
+    for form in FORMS:
+        batch, tables, q, pools = _step(form, D, device)
+        for window in (0, 20):
+            want = paged_attention_4bit(q, *pools, batch, D ** -0.5, window)
+            for seq in range(batch.num_seqs):
+                lo, hi, start = batch.cu_host[seq], batch.cu_host[seq + 1], batch.start_host[seq]
+                at = torch.arange(start, start + hi - lo, device=device)
+                for i in {0, start // PAGE, len(tables[seq]) - 1, max(0, start - 20) // PAGE}:
+                    held = batch.block_tables[seq, i].item()
+                    batch.block_tables[seq, i] = page
+                    got = paged_attention_4bit(q, *pools, batch, D ** -0.5, window)
+                    batch.block_tables[seq, i] = held
+                    sees = torch.zeros(len(q), dtype=torch.bool, device=device)
+                    sees[lo:hi] = (at >= i * PAGE) & ((at - (i + 1) * PAGE + 1 < window) | (window == 0))
+                    assert torch.equal(got[~sees], want[~sees]) and got[sees].isnan().all(), (form, window, seq, i)
+
+
+@sizes
 @pytest.mark.parametrize("code,byte", FINITE)
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 def test_the_largest_values_that_are_finite(code, byte, device, D):
