@@ -105,6 +105,8 @@ class SpeculativeEngine:
     def __init__(self, target: LlamaForCausalLM, draft: LlamaForCausalLM,
                  config: Optional[InferenceConfig] = None, gamma: int = 4):
         self.config = config or InferenceConfig()
+        if self.config.kv_cache_bits != 16:
+            raise ValueError("4-bit caches are paged: ContinuousBatchEngine serves them")
         self.gamma = gamma
         self.target = _CachedModel(target, self.config.max_seq_len)
         self.draft = _CachedModel(draft, self.config.max_seq_len)
@@ -308,6 +310,8 @@ class BatchedSpeculativeEngine:
     def __init__(self, target: LlamaForCausalLM, draft: LlamaForCausalLM,
                  config: Optional[InferenceConfig] = None, gamma: int = 4):
         self.config = config or InferenceConfig()
+        if self.config.kv_cache_bits != 16:
+            raise ValueError("4-bit caches are paged: ContinuousBatchEngine serves them")
         self.gamma = gamma
         self._target_model = target
         self._draft_model = draft

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from colossalai_amd.inference import ContinuousBatchEngine, GenerationConfig, InferenceConfig, KVCacheManager, LLMEngine
+from colossalai_amd.inference.spec_decode import BatchedSpeculativeEngine, GlideSpeculativeEngine, SpeculativeEngine
 from colossalai_amd.models import LlamaConfig, LlamaForCausalLM
 
 gpu = pytest.mark.gpu
@@ -155,3 +156,10 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
     assert [t.shape for t in kv.gather_contiguous(0, 0, 20)] == [(20, 2, 64)] * 2
+
+
+@pytest.mark.parametrize("engine", [SpeculativeEngine, BatchedSpeculativeEngine, GlideSpeculativeEngine])
+def test_engines_with_caches_of_their_own_refuse_4_bits(engine):
+    model = _model(False)
+    with pytest.raises(ValueError):
+        engine(model, model, config=InferenceConfig(kv_cache_bits=4))
