@@ -10,7 +10,7 @@ stream in the moment blocks are available — throughput is bounded by the
 8 TB/s KV stream, not by the longest member of a static batch.
 
 Llama-family models whose query and key heads are normed, and caches in 4 bits (``kv_cache_bits=4``), take
-the same steps with their tokens packed: ``paged_kv_append`` norms, rotates and writes them, and
+steps of packed tokens, prompt portions beside single tokens within ``max_step_tokens``: ``paged_kv_append`` norms, rotates and writes them, and
 attention reads the cache (``paged_attention`` / ``paged_attention_4bit``).
 
 Models that declare ``serves_ragged`` (hybrids of paged attention and
@@ -92,6 +92,8 @@ class ContinuousBatchEngine:
 
     # -------------------------------------------------------------- requests
     def add_request(self, prompt: List[int], max_new_tokens: Optional[int] = None) -> int:
+        if not len(prompt):  # steps would wait for its first token for ever
+            raise ValueError("a prompt has one token at least")
         return self.rm.add_request(list(prompt), max_new_tokens or self._gen.max_new_tokens)
 
     # ---------------------------------------------------------- ragged step
@@ -226,12 +228,12 @@ class ContinuousBatchEngine:
         requests that finished during this step."""
         if self.ragged:
             return self._step_ragged()
+        if self.packed:
+            return self._step_packed()
         gen, cfg = self._gen, self.config
         finished: Dict[int, List[int]] = {}
 
         admitted = self.rm.schedule()
-        if self.packed:
-            return self._step_packed(admitted)
         if admitted:
             prompts = [r.prompt for r in admitted]
             lens = torch.tensor([len(p) for p in prompts], device=self.device, dtype=torch.int32)
@@ -262,23 +264,24 @@ class ContinuousBatchEngine:
                     finished[r.request_id] = r.tokens
         return finished
 
-    def _step_packed(self, admitted) -> Dict[int, List[int]]:
-        """``step()`` with packed tokens: the prompts of the requests admitted, then one token of every running request."""
+    def _step_packed(self) -> Dict[int, List[int]]:
+        """``step()`` with packed tokens: one token of every sequence whose prompt is cached, and portions of the others' prompts in what is left
+        of ``max_step_tokens``."""
         gen, cfg = self._gen, self.config
         finished: Dict[int, List[int]] = {}
-
-        def advance(requests, items):
-            tokens = LLMEngine._sample(self._forward_packed(items), gen).tolist()
-            for r, token in zip(requests, tokens):
+        plan = self.rm.schedule_chunks(self.max_step_tokens)
+        if not plan:
+            return finished
+        logits = self._forward_packed([(r.request_id, tokens, r.num_computed) for r, tokens in plan])
+        for r, tokens in plan:
+            r.num_computed += len(tokens)
+        ends = [i for i, (r, _) in enumerate(plan) if r.num_computed == r.seq_len]  # a prompt's other portions choose no token
+        if ends:
+            for i, token in zip(ends, LLMEngine._sample(logits[ends] if len(ends) < len(plan) else logits, gen).tolist()):
+                r = plan[i][0]
                 self.rm.append_token(r, int(token), cfg.eos_token_id, cfg.max_seq_len)
                 if r.status.value == "finished":
                     finished[r.request_id] = r.tokens
-
-        if admitted:
-            advance(admitted, [(r.request_id, r.prompt, 0) for r in admitted])
-        running = list(self.rm.running)
-        if running:
-            advance(running, [(r.request_id, r.tokens[-1:], r.seq_len - 1) for r in running])
         return finished
 
     # ----------------------------------------------------------- convenience

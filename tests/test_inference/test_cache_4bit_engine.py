@@ -163,3 +163,30 @@ def test_engines_with_caches_of_their_own_refuse_4_bits(engine):
     model = _model(False)
     with pytest.raises(ValueError):
         engine(model, model, config=InferenceConfig(kv_cache_bits=4))
+
+
+@pytest.mark.parametrize("norm,bits", [(True, 16), (True, 4), (False, 4)])
+@pytest.mark.parametrize("budget", [1, 7, 64])
+def test_steps_keep_to_their_budget(norm, bits, budget, monkeypatch):
+    """No step runs more tokens than the budget (but one of every sequence that decodes); portions over what is cached, beside single tokens, give
+    what the plain forward does."""
+    model = _model(norm)
+    engine = _engine(model, bits, block_size=16, max_step_tokens=budget)
+    forward, steps = engine._forward_packed, []
+    monkeypatch.setattr(engine, "_forward_packed", lambda items: steps.append([(len(t), n) for _, t, n in items]) or forward(items))
+    out = engine.generate(PROMPTS, GenerationConfig(max_new_tokens=6))
+    for p, o in zip(PROMPTS, out):
+        logits = _plain_logits(model, o[:-1], bits == 4)
+        assert o[len(p):] == logits[len(p) - 1:].argmax(-1).tolist() and len(o) == len(p) + 6
+    assert all(sum(n for n, _ in step) <= max(budget, len(step)) for step in steps)
+    assert budget == 1 or any(n > 1 and at > 0 for step in steps for n, at in step)
+    assert budget == 1 or any({n > 1 for n, _ in step} == {True, False} for step in steps)
+    assert engine.kv.free_blocks == engine.kv.num_blocks
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_empty_prompts_are_refused(norm):
+    engine = _engine(_model(norm), 16)
+    with pytest.raises(ValueError):
+        engine.generate([[]])
+    assert not engine.rm.has_work and engine.generate([[3]], GenerationConfig(max_new_tokens=2))[0][0] == 3
