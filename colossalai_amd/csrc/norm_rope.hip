@@ -377,9 +377,12 @@ std::vector<at::Tensor> norm_rope_bwd(at::Tensor dq_in, at::Tensor dk_in, at::Te
     TORCH_CHECK(t.device() == x.device() && t.scalar_type() == x.scalar_type() && t.numel() == h.tokens * h.D * (t.is_same(dq) ? Hq : Hkv),
                 "qkv_norm_rope: gradients have the outputs' shapes and type");
   const auto dx = at::empty({x.size(0), x.size(1), x.size(2)}, x.options()), dwq = at::empty_like(wq), dwk = at::empty_like(wk);
-  // Three tokens a wave make up for a block's weights and sums, while there are blocks for every CU. Three waves a SIMD are 768 blocks, 384 of
-  // each kind, at once: a few more would wait for all of them (5003 tokens of 20 heads of 96 in float32: 28 us with 384 and fewer, 36 with 417),
-  // many even the kinds' shares out (4 x 8192 tokens, 32/8 heads of 128: 1024 236 us, 384 of each 325)
+  // Three tokens a wave make up for a block's weights and sums, while there are blocks for every CU. Three waves a SIMD, which every type and
+  // head size has the registers for (150 to 168), are 768 blocks, 384 of each kind, at once: a few more would wait for all of them. With 384, and with
+  // the 391, 475 and 571 of 4700, 5700 and 6850 tokens: 16/4 heads of 64 in bfloat16 20 to 24 us and 27 to 29, 8/8 of 128 23 to 29 and 28 to 32, 32/8
+  // of 128 38 to 49 and 38 to 51, 16/4 of 256 39 to 51 and 40 to 53, 4/2 of 512 in float16 29 to 37 and 36 to 43, in float32 12/4 of 96 27 to 36 and
+  // 33 to 39, 16/4 of 32 20 to 24 and 27 to 29, 32/8 of 128 the same. Many even the kinds' shares out (4 x 8192 tokens, 32/8 heads of 128: 1024 236
+  // us, 384 of each 325)
   const long one = (h.tokens + NR_WAVES - 1) / NR_WAVES, some = std::min<long>({one, 1024, std::max<long>(256, one / 3)});
   const int grid = (int)(some > 384 && some < 576 ? 384 : some);
   const auto part = at::empty({(long)grid * 2 * h.D}, x.options().dtype(at::kFloat));

@@ -10,7 +10,8 @@
 // One pass over the keys with a running reference and sum a row; a row's weights may pass its reference by 2^8 before sums are scaled anew.
 // For the product a weight is two bfloat16 pieces, 16 of its 24 bits, in every form, so that a token's result does not depend on which one it is given
 // (one piece leaves 2^-8 of each term, which shows where terms cancel: portions took 205 us for 268); their sum is that of the float32 ones.
-// What no row sees is taken out of the values too: its scale is set to 0, so that nothing behind a sequence's end shows.
+// What no row sees is taken out of the values too: its scale's byte is set to 0, the smallest and finite, so that a weight of 0 hides whatever lies
+// behind a sequence's end.
 //
 // Three forms, by the rows that a sequence's new tokens make:
 //   up to 16, or 17 to 95: a wave works alone, from memory to registers, and a block's waves take its steps in turn; their states meet in

@@ -1,5 +1,6 @@
 // The work of a step's attention, tile by tile and part by part, from the step's lengths (host only). RaggedBatch.row_plan says what it means.
-// As array operations in Python it took the host 100 to 250 us a step, here 2 to 10.
+// As array operations in Python it took the host 100 to 250 us a step, here 2 to 10; with the pinned memory and the copy to the GPU 9 to 17 us, where it
+// is to be there for every stream 28 to 37.
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -22,8 +23,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // The longest part, in steps, that tiles are cut into, `least` at least and MOST_PARTS of a tile at most: where their blocks leave some of the `most`
 // that a chip holds at once, the smallest parts that still are all at once; else twice a block's share of all steps, so that tiles are cut that the
-// others would wait for (one of 131072 beside 199 of 1024, 32/8 heads of 128: 81 us for 933; 500 tokens over 32000 beside eight over 1000: 388 for 660;
-// 200 of 1024, none cut: 44). At once the share 83 and 373, but 3000 new tokens 101 for 82: parts to join; at four times 118 and 660.
+// others would wait for (one of 131072 beside 199 of 1024, 32/8 heads of 128: 82 us for 936; 500 tokens over 32000 beside eight over 1000: 472 for 812;
+// 200 of 1024, none cut: 43). At once the share 83 and 445 to 488, but 3000 new tokens 124 for 106: parts to join; at four times 120 and 814.
 int64_t longest_part(const std::vector<Tile>& tiles, int64_t blocks_each, int64_t most, int64_t least) {
   int64_t hi = 0, total = 0;
   for (const Tile& t : tiles) {
@@ -59,7 +60,9 @@ std::tuple<at::Tensor, std::vector<int64_t>> row_plan(const std::vector<int64_t>
     few += kind[i] == 0;
     second += kind[i] == 1;
   }
-  if (second > 0 && few * heads < blocks[0] / 2)   // one launch: there is room beside the others
+  // One launch, where there is room beside the others (10 tokens over 2000 beside 31 single ones over 4000: 39 us, in two launches 43; three of 8 over 300
+  // beside ten single ones over 500: 11 and 19). Weights are as precise in every kind of tile.
+  if (second > 0 && few * heads < blocks[0] / 2)
     for (int& k : kind) k = k == 0 ? 1 : k;
   for (int64_t i = 0; i < B; ++i) {
     const int64_t per = std::max<int64_t>(1, rows[kind[i]] / group), shift = start[i] - cu[i];
