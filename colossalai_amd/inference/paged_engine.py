@@ -92,9 +92,10 @@ class ContinuousBatchEngine:
 
     # -------------------------------------------------------------- requests
     def add_request(self, prompt: List[int], max_new_tokens: Optional[int] = None) -> int:
-        if not len(prompt):  # steps would wait for its first token for ever
+        prompt = list(prompt)
+        if not prompt:  # steps would wait for its first token for ever
             raise ValueError("a prompt has one token at least")
-        return self.rm.add_request(list(prompt), max_new_tokens or self._gen.max_new_tokens)
+        return self.rm.add_request(prompt, max_new_tokens or self._gen.max_new_tokens)
 
     # ---------------------------------------------------------- ragged step
     def open_sequence(self, seq_id) -> None:
@@ -296,6 +297,8 @@ class ContinuousBatchEngine:
             prompts = [row.tolist() for row in input_ids]
         else:
             prompts = [list(p) for p in input_ids]
+        if not all(prompts):  # ahead of the first request
+            raise ValueError("a prompt has one token at least")
         ids = [self.add_request(p, self._gen.max_new_tokens) for p in prompts]
         results: Dict[int, List[int]] = {}
         while self.rm.has_work:

@@ -190,3 +190,15 @@ def test_empty_prompts_are_refused(norm):
     with pytest.raises(ValueError):
         engine.generate([[]])
     assert not engine.rm.has_work and engine.generate([[3]], GenerationConfig(max_new_tokens=2))[0][0] == 3
+
+
+def test_prompts_come_all_or_none():
+    """An empty prompt leaves no other one of its call behind; any iterable of tokens is a prompt."""
+    engine = _engine(_model(True), 16)
+    with pytest.raises(ValueError):
+        engine.generate([[3, 4], []])
+    assert not engine.rm.has_work
+    engine.add_request(iter([5, 6]), 1)
+    while engine.rm.has_work:
+        engine.step()
+    assert engine.kv.free_blocks == engine.kv.num_blocks
